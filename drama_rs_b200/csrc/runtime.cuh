@@ -29,6 +29,8 @@ namespace pf { static cudaError_t configure_all(); }
 namespace moe { static cudaError_t configure_all(); namespace f8 { static cudaError_t configure_all(); } }
 namespace stack { static cudaError_t configure_all(); }
 namespace pft { static cudaError_t configure_all(); }
+namespace bn { static cudaError_t configure_all(); }
+namespace few { static cudaError_t configure_all(); }
 
 namespace rt {
 
@@ -54,6 +56,8 @@ static cudaError_t setup(int d) {
   if ((e = moe::f8::configure_all()) != cudaSuccess) return e;
   if ((e = stack::configure_all()) != cudaSuccess) return e;
   if ((e = pft::configure_all()) != cudaSuccess) return e;
+  if ((e = bn::configure_all()) != cudaSuccess) return e;
+  if ((e = few::configure_all()) != cudaSuccess) return e;
   dv.ready = true;
   g_dev[d] = dv;
   g_ready[d].store(true, std::memory_order_release);

@@ -93,6 +93,9 @@ SIGNATURES: dict[str, tuple] = {
     "drb_router_logits": (I32, [P, P, P, I32, I32, I32, F32, P]),
     "drb_quant_q4": (I32, [P, SZ, P, P, P]),
     "drb_quant_q8": (I32, [P, SZ, P, P, P]),
+    "drb_moe_few_workspace_bytes": (I32, [I32, I32]),
+    "drb_moe_few": (I32, [P, P, P, P, I32, I32, I32, I32, I32, F32, P, P]),
+    "drb_block_norms": (I32, [P, I32, P, P, P, F32, P, P, P, P, I32, I32, I32, F32, P]),
     "drb_init": (I32, []),
     "drb_device_error": (I32, [C.POINTER(U32)]),
     "drb_test_wait_runs_out": (I32, [I32, U32, P, P, P]),

@@ -291,6 +291,32 @@ int drb_ep_sync(unsigned* const* peer_flags, const unsigned* flags, int world, i
  * the layouts above (q4: 32 bytes per group, low nibble = even k, and f16 (scale, min); q8: codes and f16 scale). */
 int drb_quant_q4(const float* w, size_t groups, uint8_t* q, dr_half* sm, dr_stream st);
 int drb_quant_q8(const float* w, size_t groups, int8_t* q, dr_half* s, dr_stream st);
+/* ---- the step of several requests that decode together --------------------------------------- */
+#define DRB_F32 0
+#define DRB_BF16 1
+#define DRB_F16 2
+/* One MoE layer for n = 1 .. 16 tokens (one row per request) in ONE cooperative kernel: y = x + moe(rmsnorm(x, post_norm)) over [n, h]
+ * f32 rows, as dr_router_topk + dr_moe_decode compute it for one (routing on fp32 logits, ties to the lower index; activations as 24-bit block
+ * fixed point, exact sums over 64 inputs). y may be x. w: host struct of device pointers. live: n device bytes or NULL; a row whose byte is
+ * 0 is not computed, costs no expert and leaves its row of y as it was (a batch captured for more requests than are there). A row with a NaN
+ * or an infinity comes out as NaNs and touches no other row. No result depends on the other rows of the call beyond the order of fp32 sums.
+ * workspace: drb_moe_few_workspace_bytes(n, topk) device bytes, 256-byte aligned, ZEROED ONCE before the first call; every
+ * call leaves it ready for the next, which may have any n, e and topk that fit it (it holds a call counter, so calls captured in several
+ * graphs may share it; calls that share it must not overlap on the GPU). After a wait that ran out (drb_device_error() != 0) zero it again.
+ * 1 <= topk <= 8, topk <= e <= 256, n <= 16, h == 2048, i == 512, at least 144 multiprocessors, no pointer but live NULL, else -1; weights and x
+ * 16-byte aligned, else -3. drb_moe_few_workspace_bytes returns -1 for an n or topk out of range. */
+int drb_moe_few_workspace_bytes(int n, int topk);
+int drb_moe_few(const drb_moe_layer* w, const float* x, float* y, const uint8_t* live, int n, int e, int topk, int h, int i, float eps,
+                void* workspace, dr_stream st);
+/* The norms between two blocks with the gate and the scaled residual between them, in one pass over [rows, d]:
+ *   t = rmsnorm(o, post_w, eps) (o itself when post_w is NULL); x_out = alpha * x + sigmoid(gate[row]) * scale[c] * t (gate [rows] and
+ *   scale [d]: NULL = 1); h = rmsnorm(x_out, pre_w, eps) (pre_w NULL: no h is written and h may be NULL).
+ * o of o_type and h of h_type (DRB_F32, DRB_BF16, DRB_F16; an fp16 h is clamped to +-65504, a NaN stays one), everything else f32. Sums in
+ * fp32; a row's result does not depend on the number of rows. x_out may be x, and h may be o when their types are of one size.
+ * 1 <= d <= 8192, else -1; any alignment of a value's own size (-3 otherwise), 16-byte aligned buffers and d % 8 == 0 are fastest.
+ * All operands, weights too, may be the work of the launch before. */
+int drb_block_norms(const void* o, int o_type, const float* post_w, const float* gate, const float* scale, float alpha, const float* x,
+                    float* x_out, const float* pre_w, void* h, int h_type, int rows, int d, float eps, dr_stream st);
 int dr_stream_destroy(dr_stream s);
 int dr_cublas_destroy(void* h);
 int drb_init(void);                    /* per-device setup; also run by the pre-capture hooks above */

@@ -1,0 +1,93 @@
+"""drb_moe_few (one MoE layer for 1 to 16 tokens) against the fp64 block.
+
+Tolerance of a row, relative to its 2-norm, with u = 2^-24 and inputs of independent signs, whose roundings add up in quadrature: an input is
+off by half a digit, at most u times the largest of 64 neighbours (3.5 times their rms at most here), and a sum over 2048 products meets three fp32 roundings
+a group of 64, each of at most u times a partial sum: 3.5 u + sqrt(3 * 32) u < 13.4 u a projection. SwiGLU multiplies two of them (silu's slope
+is below 1.1), down adds a third, the routing weights and the norm two of that size at most: 5 * 13.4 u = 4e-6.
+"""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from drama_rs_b200 import ffi, synth
+from drama_rs_b200.gpu import DevBuf, Graph, Stream, launched
+from drama_rs_b200.model import MoeLayer
+from oracle import moe_oracle as orc
+from tests.helpers import device_error_word
+
+pytestmark = pytest.mark.gpu
+H, I, EPS = 2048, 512, 1e-6
+REL = 4e-6
+
+
+class Few:
+    def __init__(self, host, n, topk, st):
+        self.l, self.st, self.n, self.topk = ffi.lib(), st, n, topk
+        self.dev = MoeLayer.upload(host, st)
+        d = self.dev
+        self.w = ffi.MoeLayerPtrs(*[t.ptr for t in (d.router, d.post_norm, d.gate_up.q, d.gate_up.sm, d.down.q, d.down.sm, d.shared_gate_up.q,
+                                                    d.shared_gate_up.s, d.shared_down.q, d.shared_down.s)])
+        self.ws = DevBuf.zeros(self.l.drb_moe_few_workspace_bytes(n, topk), st)
+
+    def call(self, x, y, live=None, n=None, topk=None):
+        return self.l.drb_moe_few(C.byref(self.w), x.at(0), y.at(0), live.at(0) if live is not None else None, self.n if n is None else n,
+                                  self.dev.experts, self.topk if topk is None else topk, H, I, EPS, self.ws.at(0), self.st.raw)
+
+    def run(self, x, live=None, in_place=False, topk=None):
+        n = x.shape[0]
+        dx = DevBuf.from_array(x.astype(np.float32), self.st)
+        dy = dx if in_place else DevBuf.from_array(np.full((n, H), 7.0, np.float32), self.st)
+        dl = DevBuf.from_array(np.asarray(live, np.uint8), self.st) if live is not None else None
+        launched(self.call(dx, dy, dl, n, topk), "moe_few")
+        return dy.download(np.float32, n * H, self.st).reshape(n, H)
+
+
+def reference(host, x, topk):
+    return orc.moe_layer(host, x, topk, EPS, np.float64)[0]
+
+
+def assert_rows(y, ref, rows):
+    for r in rows:
+        rel = np.linalg.norm(y[r] - ref[r]) / np.linalg.norm(ref[r])
+        assert rel <= REL, (r, rel)
+
+
+_LAYERS = {}
+
+
+def layer(e):
+    if e not in _LAYERS:
+        _LAYERS[e] = synth.make_layer(11 + e, synth.MoeShape(experts=e))
+    return _LAYERS[e]
+
+
+@pytest.mark.parametrize("e,n,topk", [(16, 1, 8), (16, 2, 8), (16, 3, 1), (16, 16, 8), (33, 5, 3), (8, 9, 8), (1, 4, 1), (1, 16, 1), (64, 8, 6),
+                                      (64, 12, 2), (64, 7, 8), (64, 4, 8), (64, 13, 8)])
+def test_against_the_block(e, n, topk):
+    st = Stream()
+    few = Few(layer(e), n, topk, st)
+    x = synth.make_x(e + n, n, H)
+    ref = reference(layer(e), x, topk)
+    y = few.run(x)
+    assert_rows(y, ref, range(n))
+    for _ in range(3):  # the workspace is ready for the next call, and the same call gives the same bits
+        assert np.array_equal(few.run(x), y)
+    assert np.array_equal(few.run(x, in_place=True), y)
+    assert device_error_word() == 0
+
+
+@pytest.mark.parametrize("n,live", [(1, [0]), (2, [0, 1]), (5, [1, 0, 0, 1, 0]), (16, [0] * 15 + [1]), (16, [1, 0] * 8), (9, [0] * 9)])
+def test_idle_rows_stay_as_they_were(n, live):
+    st = Stream()
+    few = Few(layer(16), n, 8, st)
+    x = synth.make_x(3 * n, n, H)
+    x[[i for i in range(n) if not live[i]]] = np.nan  # whatever an idle row holds
+    ref = reference(layer(16), np.nan_to_num(x), 8)
+    y = few.run(x, live)
+    rows = [i for i in range(n) if live[i]]
+    assert_rows(y, ref, rows)
+    assert (y[[i for i in range(n) if not live[i]]] == 7.0).all()
+    assert np.array_equal(few.run(x, live), y)
+    assert device_error_word() == 0
