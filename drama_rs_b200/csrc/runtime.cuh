@@ -31,6 +31,7 @@ namespace stack { static cudaError_t configure_all(); }
 namespace pft { static cudaError_t configure_all(); }
 namespace bn { static cudaError_t configure_all(); }
 namespace few { static cudaError_t configure_all(); }
+namespace pl { static cudaError_t configure_all(); }
 
 namespace rt {
 
@@ -58,6 +59,7 @@ static cudaError_t setup(int d) {
   if ((e = pft::configure_all()) != cudaSuccess) return e;
   if ((e = bn::configure_all()) != cudaSuccess) return e;
   if ((e = few::configure_all()) != cudaSuccess) return e;
+  if ((e = pl::configure_all()) != cudaSuccess) return e;
   dv.ready = true;
   g_dev[d] = dv;
   g_ready[d].store(true, std::memory_order_release);

@@ -95,6 +95,7 @@ SIGNATURES: dict[str, tuple] = {
     "drb_quant_q8": (I32, [P, SZ, P, P, P]),
     "drb_moe_few_workspace_bytes": (I32, [I32, I32]),
     "drb_moe_few": (I32, [P, P, P, P, I32, I32, I32, I32, I32, F32, P, P]),
+    "drb_proj_q8_lora": (I32, [P, P, P, I32, P, P, P, P, I32, I32, P, P, P, I32, I32, I32, P]),
     "drb_block_norms": (I32, [P, I32, P, P, P, F32, P, P, P, P, I32, I32, I32, F32, P]),
     "drb_init": (I32, []),
     "drb_device_error": (I32, [C.POINTER(U32)]),

@@ -308,6 +308,16 @@ int drb_quant_q8(const float* w, size_t groups, int8_t* q, dr_half* s, dr_stream
 int drb_moe_few_workspace_bytes(int n, int topk);
 int drb_moe_few(const drb_moe_layer* w, const float* x, float* y, const uint8_t* live, int n, int e, int topk, int h, int i, float eps,
                 void* workspace, dr_stream st);
+/* An int8 projection of several rows with each row's low-rank adapter beside it:
+ *   y_r = W x_r (+ res_r) + scale[a] * B_a (A_a x_r), a = adapter_of[r]; a row whose a lies outside [0, adapters) has none.
+ * w, s: Q8 [n, k]; x: [rows, k] of x_type (DRB_BF16 or DRB_F16); a: bf16 [adapters, rank, k]; b: bf16 [adapters, n, rank]; scale: f32 [adapters];
+ * adapter_of: [rows], any order; res, y: f32 [rows, n], y may be res, res may be NULL; v: f32 scratch [rows, rank]. rank 0 (then a, b, scale,
+ * adapter_of and v may be NULL) is the projection alone; adapters of a smaller rank are padded with zeros. Weights are not rounded: codes meet x
+ * exactly, sums over the 128 inputs of a scale and everything behind them are f32. Two launches (one without adapters).
+ * k a multiple of 128 up to 8192, rank a multiple of 8 up to 64, n >= 1, else -1; w, x, a, b and v 16-byte aligned, else -3. w and s are read
+ * ahead of the launch before and must not be its work; everything else may be. */
+int drb_proj_q8_lora(const int8_t* w, const dr_half* s, const void* x, int x_type, const dr_bf16* a, const dr_bf16* b, const float* scale,
+                     const int* adapter_of, int adapters, int rank, const float* res, float* y, float* v, int rows, int n, int k, dr_stream st);
 /* The norms between two blocks with the gate and the scaled residual between them, in one pass over [rows, d]:
  *   t = rmsnorm(o, post_w, eps) (o itself when post_w is NULL); x_out = alpha * x + sigmoid(gate[row]) * scale[c] * t (gate [rows] and
  *   scale [d]: NULL = 1); h = rmsnorm(x_out, pre_w, eps) (pre_w NULL: no h is written and h may be NULL).

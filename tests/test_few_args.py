@@ -50,3 +50,20 @@ def test_few_workspace_sizes():
     ws = ffi.lib().drb_moe_few_workspace_bytes
     assert ws(0, 8) == -1 and ws(17, 8) == -1 and ws(1, 0) == -1 and ws(1, 9) == -1
     assert ws(16, 8) - ws(15, 8) == 9 * (2048 + 512) * 4 and ws(1, 1) > 0
+
+
+def lora(w=A, s=A, x=A, x_type=1, a=A, b=A, scale=A, who=A, adapters=2, rank=8, res=A, y=A, v=A, rows=4, n=64, k=512):
+    return ffi.lib().drb_proj_q8_lora(w, s, x, x_type, a, b, scale, who, adapters, rank, res, y, v, rows, n, k, None)
+
+
+@pytest.mark.parametrize("kw", [dict(x_type=0), dict(x_type=3), dict(rows=-1), dict(n=0), dict(k=0), dict(k=64), dict(k=200), dict(k=8320), dict(rank=72),
+                                dict(rank=-8), dict(rank=12), dict(adapters=-1), dict(w=None), dict(s=None), dict(x=None), dict(y=None), dict(a=None),
+                                dict(b=None), dict(scale=None), dict(who=None), dict(v=None)])
+def test_lora_refuses_shapes_types_and_missing_buffers(kw):
+    assert lora(**kw) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(w=A + 8), dict(s=A + 1), dict(x=A + 2), dict(a=A + 8), dict(b=A + 2), dict(v=A + 4), dict(y=A + 2), dict(res=A + 1),
+                                dict(scale=A + 2), dict(who=A + 2)])
+def test_lora_refuses_misaligned_buffers(kw):
+    assert lora(**kw) == -3
