@@ -14,7 +14,7 @@
 
 namespace bn {
 
-constexpr int MAX_D = 8192;
+constexpr int MAX_D = 8192;  // eight values a thread
 enum Type { F32 = 0, BF16 = 1, F16 = 2 };
 
 struct Args {
@@ -45,127 +45,156 @@ DRB_DEV float block_sum(float v, float* red) {
   return s;
 }
 
-// A block per row. Thread t holds VEC consecutive values at (t + i * threads) * VEC, i < NCH. VEC = 8: 16-byte accesses, d a multiple
-// of 8 and every pointer aligned; VEC = 1 for any other row.
-template <int VEC, int NCH>
-__global__ void __launch_bounds__(VEC == 8 ? 256 : 1024) k_block_norms(Args a) {
+// Eight values of a row a thread: eight consecutive ones (WIDE: 16-byte accesses, d a multiple of 8 and every pointer aligned), or every
+// blockDim-th one for any other row. A block keeps its part of the weights in registers and goes through rows blockIdx, + gridDim, ...; the
+// next row is requested before the current one's sums, so that the stream does not wait for them.
+template <bool WIDE>
+struct Cols {
+  int c0, step, d;
+  DRB_DEV Cols(int d) : c0(threadIdx.x * (WIDE ? 8 : 1)), step(WIDE ? 1 : blockDim.x), d(d) {}
+  DRB_DEV bool in(int j) const { return WIDE ? c0 < d : c0 + j * step < d; }
+  DRB_DEV void load(const float* p, float (&v)[8]) const {
+    if constexpr (WIDE) {
+      if (!in(0)) return;
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(p + c0)), b = __ldcg(reinterpret_cast<const float4*>(p + c0) + 1);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (in(j)) v[j] = __ldcg(p + c0 + j * step);
+    }
+  }
+  DRB_DEV void store(float* p, const float (&v)[8]) const {
+    if constexpr (WIDE) {
+      if (!in(0)) return;
+      reinterpret_cast<float4*>(p + c0)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p + c0)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (in(j)) p[c0 + j * step] = v[j];
+    }
+  }
+  // 16-bit values stay as they are until they are used: w[j] holds values 2 j and 2 j + 1
+  DRB_DEV void load16(const uint16_t* p, uint32_t (&w)[4]) const {
+    if constexpr (WIDE) {
+      if (!in(0)) return;
+      const uint4 a = __ldcg(reinterpret_cast<const uint4*>(p + c0));
+      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = in(2 * j) ? __ldcg(p + c0 + 2 * j * step) : 0u, hi = in(2 * j + 1) ? __ldcg(p + c0 + (2 * j + 1) * step) : 0u;
+        w[j] = lo | hi << 16;
+      }
+    }
+  }
+  DRB_DEV void store16(uint16_t* p, const float (&v)[8], int type) const {
+    if constexpr (WIDE) {
+      if (!in(0)) return;
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = (uint32_t)narrow(v[2 * j], type) | (uint32_t)narrow(v[2 * j + 1], type) << 16;
+      *reinterpret_cast<uint4*>(p + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (in(j)) p[c0 + j * step] = narrow(v[j], type);
+    }
+  }
+};
+
+template <bool WIDE, bool O16, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1) k_block_norms(Args a, int rows) {
   __shared__ float red[2][32];
-  const int d = a.d, step = (int)blockDim.x * VEC, c0 = (int)threadIdx.x * VEC;
-  const size_t row = (size_t)blockIdx.x * d;
+  const int d = a.d;
+  const Cols<WIDE> cols(d);
   pdl_launch_dependents();
   pdl_wait();
-  float t[NCH][VEC], x[NCH][VEC];
+  float xn[8] = {}, on[8] = {}, gn = 0.f;
+  uint32_t hn[4] = {};
+  auto fetch = [&](int row) {
+    const size_t at = (size_t)row * d;
+    cols.load(a.x + at, xn);
+    if constexpr (O16) cols.load16(static_cast<const uint16_t*>(a.o) + at, hn);
+    else cols.load(static_cast<const float*>(a.o) + at, on);
+    if (a.gate) gn = __ldcg(a.gate + row);
+  };
+  fetch(blockIdx.x);
+  float wt[8], wn[8] = {};  // post_w * scale, pre_w
+  {
+    float w[8], s[8];
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = c0 + i * step;
+    for (int j = 0; j < 8; ++j) w[j] = s[j] = 1.f;
+    if (a.post_w) cols.load(a.post_w, w);
+    if (a.scale) cols.load(a.scale, s);
+    if (a.pre_w) cols.load(a.pre_w, wn);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) t[i][j] = 0.f, x[i][j] = 0.f;
-    if (c >= d) continue;
-    if constexpr (VEC == 8) {
-      const float4* xp = reinterpret_cast<const float4*>(a.x + row + c);
-      const float4 x0 = __ldcg(xp), x1 = __ldcg(xp + 1);
-      x[i][0] = x0.x, x[i][1] = x0.y, x[i][2] = x0.z, x[i][3] = x0.w, x[i][4] = x1.x, x[i][5] = x1.y, x[i][6] = x1.z, x[i][7] = x1.w;
-      if (a.o_type == F32) {
-        const float4* op = reinterpret_cast<const float4*>(static_cast<const float*>(a.o) + row + c);
-        const float4 o0 = __ldcg(op), o1 = __ldcg(op + 1);
-        t[i][0] = o0.x, t[i][1] = o0.y, t[i][2] = o0.z, t[i][3] = o0.w, t[i][4] = o1.x, t[i][5] = o1.y, t[i][6] = o1.z, t[i][7] = o1.w;
-      } else {
-        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o) + row + c));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t[i][2 * j] = widen((uint16_t)w[j], a.o_type), t[i][2 * j + 1] = widen((uint16_t)(w[j] >> 16), a.o_type);
-      }
-    } else {
-      x[i][0] = __ldcg(a.x + row + c);
-      t[i][0] = a.o_type == F32 ? __ldcg(static_cast<const float*>(a.o) + row + c)
-                                : widen(__ldcg(static_cast<const uint16_t*>(a.o) + row + c), a.o_type);
-    }
+    for (int j = 0; j < 8; ++j) wt[j] = w[j] * s[j];
   }
-  float f = 1.f;
-  if (a.post_w) {
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const size_t at = (size_t)row * d;
+    float x[8], t[8];
+    const float gate = gn;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = xn[j];
+      if constexpr (O16) t[j] = widen((uint16_t)(hn[j / 2] >> (j & 1 ? 16 : 0)), a.o_type);
+      else t[j] = on[j];
+    }
+    if (row + (int)gridDim.x < rows) fetch(row + gridDim.x);
+    float f = 1.f;
+    if (a.post_w) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(t[j], t[j], ss);
+      f = rsqrtf(block_sum(ss, red[0]) / (float)d + a.eps);
+    }
+    if (a.gate) f *= sigmoid_f(gate);
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(f, t[j] * wt[j], a.alpha * x[j]), ss = fmaf(x[j], x[j], ss);
+    cols.store(a.x_out + at, x);
+    if (a.pre_w) {
+      const float r = rsqrtf(block_sum(ss, red[1]) / (float)d + a.eps);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) ss = fmaf(t[i][j], t[i][j], ss);
-    f = rsqrtf(block_sum(ss, red[0]) / (float)d + a.eps);
-  }
-  if (a.gate) f *= sigmoid_f(__ldcg(a.gate + blockIdx.x));
-  auto weights = [&](const float* w, int c, float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-      const float4 w0 = __ldcg(reinterpret_cast<const float4*>(w + c)), w1 = __ldcg(reinterpret_cast<const float4*>(w + c) + 1);
-      v[0] = w0.x, v[1] = w0.y, v[2] = w0.z, v[3] = w0.w, v[4] = w1.x, v[5] = w1.y, v[6] = w1.z, v[7] = w1.w;
-    } else {
-      v[0] = __ldcg(w + c);
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * r * wn[j];
+      if (a.h_type == F32) cols.store(static_cast<float*>(a.h) + at, x);
+      else cols.store16(static_cast<uint16_t*>(a.h) + at, x, a.h_type);
     }
-  };
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = c0 + i * step;
-    if (c >= d) continue;
-    float w[VEC];
-    if (a.post_w) {
-      weights(a.post_w, c, w);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) t[i][j] *= w[j];
-    }
-    if (a.scale) {
-      weights(a.scale, c, w);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) t[i][j] *= w[j];
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) x[i][j] = fmaf(f, t[i][j], a.alpha * x[i][j]), ss = fmaf(x[i][j], x[i][j], ss);
-    if constexpr (VEC == 8) {
-      float4* xp = reinterpret_cast<float4*>(a.x_out + row + c);
-      xp[0] = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-      xp[1] = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
-    } else {
-      a.x_out[row + c] = x[i][0];
-    }
-  }
-  if (!a.pre_w) return;
-  const float r = rsqrtf(block_sum(ss, red[1]) / (float)d + a.eps);
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = c0 + i * step;
-    if (c >= d) continue;
-    float w[VEC];
-    weights(a.pre_w, c, w);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) w[j] = x[i][j] * r * w[j];
-    if constexpr (VEC == 8) {
-      if (a.h_type == F32) {
-        float4* hp = reinterpret_cast<float4*>(static_cast<float*>(a.h) + row + c);
-        hp[0] = make_float4(w[0], w[1], w[2], w[3]);
-        hp[1] = make_float4(w[4], w[5], w[6], w[7]);
-      } else {
-        uint32_t p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = (uint32_t)narrow(w[2 * j], a.h_type) | (uint32_t)narrow(w[2 * j + 1], a.h_type) << 16;
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row + c) = make_uint4(p[0], p[1], p[2], p[3]);
-      }
-    } else {
-      if (a.h_type == F32) static_cast<float*>(a.h)[row + c] = w[0];
-      else static_cast<uint16_t*>(a.h)[row + c] = narrow(w[0], a.h_type);
-    }
+    // a warp writes its slot of one sum again only behind the other sum's barrier; with one sum a row it has to be kept apart
+    if (!a.post_w || !a.pre_w) __syncthreads();
   }
 }
 
-template <int VEC, int NCH>
-static void launch(const Args& a, int rows, cudaStream_t st, bool pdl) {
-  const int threads = ((a.d + VEC * NCH - 1) / (VEC * NCH) + 31) / 32 * 32;
-  drb_launch(k_block_norms<VEC, NCH>, dim3(rows), dim3(threads), 0, st, pdl, a);
+// As many blocks as are resident at once go through the rows together.
+template <bool WIDE, bool O16, int MAXT>
+static void launch(const Args& a, int rows, cudaStream_t st, const DrbDevice& dev) {
+  const int threads = ((a.d + 7) / 8 + 31) / 32 * 32;
+  const int fit = dev.sms * (MAXT == 256 ? 768 / threads : 1);
+  drb_launch(k_block_norms<WIDE, O16, MAXT>, dim3(rows < fit ? rows : fit), dim3(threads), 0, st, dev.pdl, a, rows);
 }
 
+template <bool WIDE, bool O16>
+static void launch_any(const Args& a, int rows, cudaStream_t st, const DrbDevice& dev) {
+  if (a.d <= 2048) launch<WIDE, O16, 256>(a, rows, st, dev);
+  else if (a.d <= 4096) launch<WIDE, O16, 512>(a, rows, st, dev);
+  else launch<WIDE, O16, 1024>(a, rows, st, dev);
+}
+
+template <bool WIDE, bool O16>
+static cudaError_t configure() {
+  cudaError_t e;
+  if ((e = drb_carveout(k_block_norms<WIDE, O16, 256>)) != cudaSuccess) return e;
+  if ((e = drb_carveout(k_block_norms<WIDE, O16, 512>)) != cudaSuccess) return e;
+  return drb_carveout(k_block_norms<WIDE, O16, 1024>);
+}
 static cudaError_t configure_all() {
   cudaError_t e;
-  if ((e = drb_carveout(k_block_norms<8, 1>)) != cudaSuccess) return e;
-  if ((e = drb_carveout(k_block_norms<8, 2>)) != cudaSuccess) return e;
-  if ((e = drb_carveout(k_block_norms<8, 4>)) != cudaSuccess) return e;
-  if ((e = drb_carveout(k_block_norms<1, 2>)) != cudaSuccess) return e;
-  return drb_carveout(k_block_norms<1, 8>);
+  if ((e = configure<true, true>()) != cudaSuccess) return e;
+  if ((e = configure<true, false>()) != cudaSuccess) return e;
+  if ((e = configure<false, true>()) != cudaSuccess) return e;
+  return configure<false, false>();
 }
 
 }  // namespace bn
@@ -182,14 +211,7 @@ extern "C" int drb_block_norms(const void* o, int o_type, const float* post_w, c
   if (rows == 0) return 0;
   const bn::Args a = {o, post_w, gate, scale, x, pre_w, x_out, h, o_type, h_type, d, alpha, eps};
   const bool wide = d % 8 == 0 && !off(o, 16) && !off(x, 16) && !off(x_out, 16) && !off(post_w, 16) && !off(scale, 16) && !off(pre_w, 16) && !(pre_w && off(h, 16));
-  if (wide) {
-    if (d <= 2048) bn::launch<8, 1>(a, rows, st, dev.pdl);
-    else if (d <= 4096) bn::launch<8, 2>(a, rows, st, dev.pdl);
-    else bn::launch<8, 4>(a, rows, st, dev.pdl);
-  } else if (d <= 2048) {
-    bn::launch<1, 2>(a, rows, st, dev.pdl);
-  } else {
-    bn::launch<1, 8>(a, rows, st, dev.pdl);
-  }
+  if (wide) o_type ? bn::launch_any<true, true>(a, rows, st, dev) : bn::launch_any<true, false>(a, rows, st, dev);
+  else o_type ? bn::launch_any<false, true>(a, rows, st, dev) : bn::launch_any<false, false>(a, rows, st, dev);
   return 0;
 }
