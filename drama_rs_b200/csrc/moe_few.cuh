@@ -38,58 +38,60 @@ using moe::H;
 using moe::I;
 
 constexpr int CW = 16, THREADS = CW * 32;
-constexpr int MAX_TOK = 16, MAX_K = 8, MAX_E = 256, MAX_HIT = MAX_TOK * MAX_K;
-constexpr int SHARED_BLOCKS = 16;             // blocks of the shared expert's gate/up: a tile for each group of four warps
+constexpr int MAX_TOK = 16, MAX_K = 8, MAX_E = 256, MAX_ENT = MAX_TOK * MAX_K;
+constexpr int TOK = 8;                          // tokens that a tile meets at once; an expert of more is two entries of the lists below
+constexpr int SHARED_BLOCKS = 16;               // blocks of the shared expert's gate/up (for each eight tokens): a tile for each four warps
 constexpr int GU_TILES = I / 8, DN_TILES = H / 16;
-constexpr int MIN_GRID = 144, MAX_GRID = 1024;  // runs of at most 64 gate/up and 128 down tiles: two experts a block
-constexpr int LOGIT_STRIDE = MAX_E + 8;       // words a token
+constexpr int MIN_GRID = 144, MAX_GRID = 1024;  // a block's share of either list spans two entries at most
+constexpr int LOGIT_STRIDE = MAX_E + 8;         // words a token
 
 // Workspace: the head is the same for every size, activations and weighted results follow.
 struct alignas(256) Head {
   unsigned epoch, seen;  // calls so far; blocks that have read `epoch` in this call
   unsigned pad[62];
-  unsigned act_done[2][MAX_HIT + 8];   // [call parity][expert hit, MAX_HIT = shared]: gate/up tiles finished; [MAX_HIT + 1]: blocks finished
+  unsigned done[2][MAX_ENT + 8];  // [call parity][counter, see below]
   unsigned long long logits[MAX_TOK * LOGIT_STRIDE];
 };
+enum Counter { SHARED_ACT = MAX_ENT, BLOCKS = MAX_ENT + 2, DIGITS };  // gate/up tiles of entry i, of the shared expert's halves; blocks
+                                                                      // finished; eighths of tokens whose digits are written
 static_assert(sizeof(Head) % 256 == 0 && offsetof(Head, logits) % 16 == 0, "aligned sections");
 
 constexpr int SUB = 2048;                // a step of a warp: 16 rows x 128 bytes
 constexpr int SLOT = SUB + 256;          // and 16 bytes of scales a row
 constexpr int PITCH = H + 64, DPITCH = I + 64;    // bytes between digit planes: neighbouring planes on different banks
+constexpr int TOKEN_PLANES = 3 * PITCH;           // a token's digits, in the workspace and in shared memory
 constexpr int MP = H / 64 + 1, DMP = I / 64 + 1;  // per 64 inputs, tokens apart: (delta, sum, 65536 delta, 0), see Cols
+constexpr int TOKEN_BYTES = TOKEN_PLANES + MP * 16;
 
-template <int TOK>
-struct Shape {
-  static constexpr int DEPTH = TOK > 8 ? 3 : 4;
-  static constexpr int PLANES = 3 * TOK * PITCH, META = TOK * MP * 16, RING = CW * DEPTH * SLOT, RED = CW * 16 * 8 * 4;
-  static constexpr int CTL = 3072;
-  static constexpr size_t BYTES = CTL + PLANES + META + RING + RED;
-  static_assert(BYTES <= 232448 && 2 * 3 * TOK * DPITCH <= PLANES && 2 * TOK * DMP * 16 <= META, "shared memory");
-};
+constexpr int DEPTH = 4;
+constexpr int CTL_BYTES = 3072, PLANES_BYTES = TOK * TOKEN_PLANES, META_BYTES = TOK * MP * 16, RING_BYTES = CW * DEPTH * SLOT, RED_BYTES = CW * 16 * 8 * 4;
+constexpr size_t SMEM_BYTES = CTL_BYTES + PLANES_BYTES + META_BYTES + RING_BYTES + RED_BYTES;
+static_assert(SMEM_BYTES <= 232448 && 2 * 3 * TOK * DPITCH <= PLANES_BYTES && 2 * TOK * DMP * 16 <= META_BYTES, "shared memory");
+static_assert((CTL_BYTES + PLANES_BYTES + META_BYTES) % 128 == 0 && SLOT % 128 == 0, "reads of the ring are told apart by their low bits");
 
-struct Seg {  // the tokens of one expert in this block's run
+struct Seg {  // the tokens of an entry in this block's run
   int count;
-  float wt[16];           // weight of the expert's result
-  float rr[16];           // 1 / rms of the token
-  short row[16];          // row of the activations and of the weighted results
-  unsigned char pos[16];  // digit planes
+  float wt[TOK];           // weight of the expert's result
+  float rr[TOK];           // 1 / rms of the token
+  short row[TOK];          // row of the activations and of the weighted results
+  unsigned char pos[TOK];  // digit planes
 };
 
 struct Ctl {
   Seg seg[2];
-  uint64_t arrived[4][4];   // [group of four warps][tile mod 4]: warps whose sums of a tile lie in shared memory
+  int arrived[4][4], finished[4];  // [group of four warps]: warps whose sums of tile t lie in shared memory (t mod 4), tiles finished
   int idx[MAX_TOK][MAX_K];
   float wts[MAX_TOK][MAX_K];
-  float sgate[MAX_TOK], rr[MAX_TOK], rr_own[MAX_TOK], ss[CW];
-  unsigned mask[MAX_E];     // tokens that chose the expert
-  unsigned char hit[MAX_HIT];
-  int wsum[8];
-  int nhit, abort;
-  int range[4];             // this block's gate/up tiles and down tiles
+  float sgate[MAX_TOK], rr[MAX_TOK];
+  unsigned mask[MAX_E];            // tokens that chose the expert
+  unsigned short ent[MAX_ENT];     // expert, + 256: its tokens from the ninth on
+  int wsum[8], range[4];           // this block's gate/up tiles and down tiles
+  int abort;
 };
-static_assert(sizeof(Ctl) <= Shape<16>::CTL, "control block");
+static_assert(sizeof(Ctl) <= CTL_BYTES, "control block");
 
 DRB_DEV void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+DRB_DEV void cp8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 DRB_DEV void cp4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 DRB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -136,15 +138,14 @@ DRB_DEV void digits4(const float4& v, unsigned char* plane, int pitch, float4* m
   if ((lane & 15) == 0) meta[lane >> 4] = make_float4(delta, sum, 65536.f * delta, 0.f);
 }
 
-// The weights of a warp's tiles on their way. A tile's rows are contiguous; the next tile of the same expert lies dp (ds) bytes on.
+// The weights of a warp's tiles on their way. The next tile of the same expert lies dp (ds) bytes on.
 enum Mode { SHARED_GU, GU, DN, OVER };
 struct Loader {
   const unsigned char *p;   // this lane's first row and piece of the next step
-  const unsigned char *sp;  // this lane's row of scales (lanes 0..15)
-  uint32_t at;              // where they go in a slot
+  const unsigned char *sp;  // this lane's row of scales
+  uint32_t at;              // where the pieces go in a slot
   int stride, gap;          // bytes over four rows, and from row r to row r + 8
-  int sub, nsub, u, uend, ustep, dp, ds, mode;
-  bool int8;
+  int sub, u, uend, ustep, dp, ds, sstep, mode;
 };
 
 struct Params {
@@ -154,40 +155,34 @@ struct Params {
   const uint8_t* live;
   Head* ws;
   float *act, *part;
+  unsigned char* digits;  // [n] x (TOKEN_PLANES, MP x 16 bytes)
   int n, e, topk;
   float eps;
   unsigned poll_limit;
 };
 
-// One warp's share of a tile: 16 rows against the tokens of a segment. TG = 0: one or two tokens, four columns each (three digits);
-// TG = 1, 2: up to 8 or 16 tokens, a column tile per digit and eight tokens.
-template <int TG>
-struct Acc {
-  float v[TG ? TG * 4 : 2];
-};
+// One warp's share of a tile: 16 rows against the tokens of an entry. TG = 0: one or two tokens, four columns each (three digits); TG = 1: up
+// to eight, a column tile per digit. The sums: rows g and g + 8, or rows g (two), g + 8 (two) of tokens 2 t, 2 t + 1.
+// Reads of shared memory by its own 32-bit addresses: behind pointers kept in structs the compiler takes generic loads.
+template <typename T>
+DRB_DEV T lds(uint32_t a) { return *static_cast<const T*>(__cvta_shared_to_generic(a)); }
 
-template <int TG>
 struct Cols {
-  const unsigned char* b[TG ? TG : 1];         // this lane's column: its token's digit planes
-  const unsigned char* m[TG ? 2 * TG : 1];     // delta and sum of the columns whose sums this lane holds. TG = 0: lanes of the third digit
-                                               // take 65536 delta and no sum
-  int second;                                  // TG = 0: weight of this lane's second column
+  uint32_t b;     // this lane's column: its token's digit planes
+  uint32_t m[2];  // delta and sum of the columns whose sums this lane holds. TG = 0: lanes of the third digit take 65536 delta and no sum
+  int second;     // TG = 0: weight of this lane's second column
 };
 
-template <int TG>
-DRB_DEV void cols_set(Cols<TG>& c, const Seg& s, const unsigned char* planes, int pitch, const float4* meta, int mp, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  if constexpr (TG == 0) {
-    c.b[0] = planes + (3 * s.pos[min(g >> 2, s.count - 1)] + min(g & 3, 2)) * pitch + 16 * t;
-    c.m[0] = reinterpret_cast<const unsigned char*>(meta + s.pos[min(t >> 1, s.count - 1)] * mp) + 8 * (t & 1);
+DRB_DEV void cols_set(Cols& c, int tg, const Seg& s, uint32_t planes, int pitch, uint32_t meta, int mp, int lane) {
+  const int g = lane >> 2, t = lane & 3, last = s.count - 1;
+  if (tg == 0) {
+    c.b = planes + (3 * s.pos[min(g >> 2, last)] + min(g & 3, 2)) * pitch + 16 * t;
+    c.m[0] = meta + s.pos[min(t >> 1, last)] * mp * 16 + 8 * (t & 1);
     c.second = t & 1 ? 0 : 256;
   } else {
-#pragma unroll
-    for (int i = 0; i < TG; ++i) {
-      c.b[i] = planes + 3 * s.pos[min(8 * i + g, s.count - 1)] * pitch + 16 * t;
-      c.m[2 * i] = reinterpret_cast<const unsigned char*>(meta + s.pos[min(8 * i + 2 * t, s.count - 1)] * mp);
-      c.m[2 * i + 1] = reinterpret_cast<const unsigned char*>(meta + s.pos[min(8 * i + 2 * t + 1, s.count - 1)] * mp);
-    }
+    c.b = planes + 3 * s.pos[min(g, last)] * pitch + 16 * t;
+    c.m[0] = meta + s.pos[min(2 * t, last)] * mp * 16;
+    c.m[1] = meta + s.pos[min(2 * t + 1, last)] * mp * 16;
   }
 }
 
@@ -200,613 +195,609 @@ DRB_DEV void mma_s8_zero(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
 // 64 inputs: A in the operand's registers, group kg of the planes; s0, m0: scale and min of row g, s1, m1 of row g + 8. A digit's sum stays
 // below 2^20.1 (int8 codes), so it and 256 times the next one's fit an integer.
 template <int TG, bool MIN>
-DRB_DEV void group64(Acc<TG>& acc, const Cols<TG>& c, int pitch, int kg, const uint32_t (&a)[8], float s0, float m0, float s1, float m1) {
+DRB_DEV void group64(float (&acc)[4], const Cols& c, int pitch, int kg, const uint32_t (&a)[8], float s0, float m0, float s1, float m1) {
   if constexpr (TG == 0) {
-    const uint4 b = *reinterpret_cast<const uint4*>(c.b[0] + 64 * kg);
+    const uint4 b = lds<uint4>(c.b + 64 * kg);
     int d[4];
     mma_s8_zero(d, a[0], a[1], a[2], a[3], b.x, b.y);
     gemv::q8::mma_s8(d, a[4], a[5], a[6], a[7], b.z, b.w);
-    const float2 m = *reinterpret_cast<const float2*>(c.m[0] + 16 * kg);
-    acc.v[0] = fmaf(s0 * m.x, (float)(d[1] * c.second + d[0]), acc.v[0]);
-    acc.v[1] = fmaf(s1 * m.x, (float)(d[3] * c.second + d[2]), acc.v[1]);
-    if (MIN) acc.v[0] = fmaf(m0, m.y, acc.v[0]), acc.v[1] = fmaf(m1, m.y, acc.v[1]);
+    const float2 m = lds<float2>(c.m[0] + 16 * kg);
+    acc[0] = fmaf(s0 * m.x, (float)(d[1] * c.second + d[0]), acc[0]);
+    acc[1] = fmaf(s1 * m.x, (float)(d[3] * c.second + d[2]), acc[1]);
+    if (MIN) acc[0] = fmaf(m0, m.y, acc[0]), acc[1] = fmaf(m1, m.y, acc[1]);
   } else {
+    int d[3][4];
 #pragma unroll
-    for (int i = 0; i < TG; ++i) {
-      int d[3][4];
+    for (int l = 0; l < 3; ++l) {
+      const uint4 b = lds<uint4>(c.b + l * pitch + 64 * kg);
+      mma_s8_zero(d[l], a[0], a[1], a[2], a[3], b.x, b.y);
+      gemv::q8::mma_s8(d[l], a[4], a[5], a[6], a[7], b.z, b.w);
+    }
+    const float2 c0 = lds<float2>(c.m[0] + 16 * kg), c1 = lds<float2>(c.m[1] + 16 * kg);
+    float f[4];
 #pragma unroll
-      for (int l = 0; l < 3; ++l) {
-        const uint4 b = *reinterpret_cast<const uint4*>(c.b[i] + l * pitch + 64 * kg);
-        mma_s8_zero(d[l], a[0], a[1], a[2], a[3], b.x, b.y);
-        gemv::q8::mma_s8(d[l], a[4], a[5], a[6], a[7], b.z, b.w);
-      }
-      const float2 c0 = *reinterpret_cast<const float2*>(c.m[2 * i] + 16 * kg), c1 = *reinterpret_cast<const float2*>(c.m[2 * i + 1] + 16 * kg);
-      float f[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = fmaf((float)d[2][j], 65536.f, (float)(d[1][j] * 256 + d[0][j]));
-      float* v = acc.v + 4 * i;
-      v[0] = fmaf(s0, f[0] * c0.x, v[0]), v[1] = fmaf(s0, f[1] * c1.x, v[1]);
-      v[2] = fmaf(s1, f[2] * c0.x, v[2]), v[3] = fmaf(s1, f[3] * c1.x, v[3]);
-      if (MIN) {
-        v[0] = fmaf(m0, c0.y, v[0]), v[1] = fmaf(m0, c1.y, v[1]);
-        v[2] = fmaf(m1, c0.y, v[2]), v[3] = fmaf(m1, c1.y, v[3]);
-      }
+    for (int j = 0; j < 4; ++j) f[j] = fmaf((float)d[2][j], 65536.f, (float)(d[1][j] * 256 + d[0][j]));
+    acc[0] = fmaf(s0, f[0] * c0.x, acc[0]), acc[1] = fmaf(s0, f[1] * c1.x, acc[1]);
+    acc[2] = fmaf(s1, f[2] * c0.x, acc[2]), acc[3] = fmaf(s1, f[3] * c1.x, acc[3]);
+    if (MIN) {
+      acc[0] = fmaf(m0, c0.y, acc[0]), acc[1] = fmaf(m0, c1.y, acc[1]);
+      acc[2] = fmaf(m1, c0.y, acc[2]), acc[3] = fmaf(m1, c1.y, acc[3]);
     }
   }
 }
 
-// One step of 128 bytes a row: 256 int4 or 128 int8 inputs from group kg on. The ring keeps 16-byte pieces where reads of 8 rows meet
-// no bank twice (see `issue`).
+// One step of 128 bytes a row: 256 int4 or 128 int8 inputs from group kg on. r0: this lane's place in the slot (see `issue`), sc: in its scales.
 template <int TG, bool INT8>
-DRB_DEV void step(Acc<TG>& acc, const Cols<TG>& c, int pitch, int kg, const unsigned char* slot, int sub, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  const unsigned char* r0 = slot + g * 128;
-  const unsigned char* r1 = r0 + 8 * 128;
+DRB_DEV void step(float (&acc)[4], const Cols& c, int pitch, int kg, uint32_t r0, uint32_t sc) {
   uint32_t a[8];
   if constexpr (INT8) {
-    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(slot + SUB + 16 * g), w1 = *reinterpret_cast<const uint32_t*>(slot + SUB + 16 * g + 128);
-    const float s0 = __half2float(__ushort_as_half((uint16_t)(sub & 1 ? w0 >> 16 : w0)));
-    const float s1 = __half2float(__ushort_as_half((uint16_t)(sub & 1 ? w1 >> 16 : w1)));
+    const float s0 = __half2float(lds<__half>(sc)), s1 = __half2float(lds<__half>(sc + 128));
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int at = 64 * (q ^ (g & 1)) + 16 * t;
-      const uint4 u = *reinterpret_cast<const uint4*>(r0 + at), v = *reinterpret_cast<const uint4*>(r1 + at);
+      const uint4 u = lds<uint4>(r0 ^ (64 * q)), v = lds<uint4>((r0 ^ (64 * q)) + 1024);
       a[0] = prmt(u.x, u.y, 0x6420u), a[1] = prmt(v.x, v.y, 0x6420u), a[2] = prmt(u.x, u.y, 0x7531u), a[3] = prmt(v.x, v.y, 0x7531u);
       a[4] = prmt(u.z, u.w, 0x6420u), a[5] = prmt(v.z, v.w, 0x6420u), a[6] = prmt(u.z, u.w, 0x7531u), a[7] = prmt(v.z, v.w, 0x7531u);
       group64<TG, false>(acc, c, pitch, kg + q, a, s0, 0.f, s1, 0.f);
     }
   } else {
-    const uint4 w0 = *reinterpret_cast<const uint4*>(slot + SUB + 16 * g), w1 = *reinterpret_cast<const uint4*>(slot + SUB + 16 * g + 128);
+    const uint4 w0 = lds<uint4>(sc), w1 = lds<uint4>(sc + 128);
     const uint32_t sm0[4] = {w0.x, w0.y, w0.z, w0.w}, sm1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int at = 32 * (q ^ (g & 3)) + 8 * t;
-      const uint2 u = *reinterpret_cast<const uint2*>(r0 + at), v = *reinterpret_cast<const uint2*>(r1 + at);
+      const uint2 u = lds<uint2>(r0 ^ (32 * q)), v = lds<uint2>((r0 ^ (32 * q)) + 1024);
       a[0] = u.x & 0x0F0F0F0Fu, a[1] = v.x & 0x0F0F0F0Fu, a[2] = (u.x >> 4) & 0x0F0F0F0Fu, a[3] = (v.x >> 4) & 0x0F0F0F0Fu;
       a[4] = u.y & 0x0F0F0F0Fu, a[5] = v.y & 0x0F0F0F0Fu, a[6] = (u.y >> 4) & 0x0F0F0F0Fu, a[7] = (v.y >> 4) & 0x0F0F0F0Fu;
-      const float2 c0 = __half22float2(*reinterpret_cast<const __half2*>(&sm0[q])), c1 = __half22float2(*reinterpret_cast<const __half2*>(&sm1[q]));
-      group64<TG, true>(acc, c, pitch, kg + q, a, c0.x, c0.y, c1.x, c1.y);
+      const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&sm0[q])), f1 = __half22float2(*reinterpret_cast<const __half2*>(&sm1[q]));
+      group64<TG, true>(acc, c, pitch, kg + q, a, f0.x, f0.y, f1.x, f1.y);
     }
   }
 }
 
-// What a tile costs with `count` tokens, in quarters of one with one or two: instructions, which grow with the column tiles.
-DRB_DEV int tile_cost(int count) { return count <= 2 ? 4 : count <= 8 ? 6 : 11; }
-constexpr int SHARED_HEAD_START = 8;  // the shared expert's gate/up, in tiles of one or two tokens that its blocks do less of
+// What a tile costs, in quarters of one with one or two tokens: instructions, which grow with the column tiles.
+DRB_DEV int tile_cost(int count) { return count <= 2 ? 4 : 6; }
+constexpr int SHARED_HEAD_START = 8;  // the shared expert's gate/up, in tiles of its number of tokens that its blocks do less of
 
-template <int TOK>
 __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
-  using S = Shape<TOK>;
-  constexpr int DEPTH = S::DEPTH;
   extern __shared__ __align__(128) unsigned char dyn[];
   Ctl& ctl = *reinterpret_cast<Ctl*>(dyn);
-  unsigned char* planes = dyn + S::CTL;
-  float4* meta = reinterpret_cast<float4*>(planes + S::PLANES);
+  unsigned char* planes = dyn + CTL_BYTES;
+  float4* meta = reinterpret_cast<float4*>(planes + PLANES_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp >> 2, kq = warp & 3;
-  unsigned char* ring = planes + S::PLANES + S::META + warp * DEPTH * SLOT;
-  float* red = reinterpret_cast<float*>(planes + S::PLANES + S::META + S::RING);
+  float* red = reinterpret_cast<float*>(planes + PLANES_BYTES + META_BYTES + RING_BYTES);
+  const uint32_t ring = smem_u32(planes) + PLANES_BYTES + META_BYTES + warp * DEPTH * SLOT, ring_end = ring + DEPTH * SLOT;
   const int n = P.n, E = P.e, topk = P.topk, E1 = E + 1;
   const int G = (int)gridDim.x, b = (int)blockIdx.x;
   volatile int* abort_flag = &ctl.abort;
-  const int GN = G - SHARED_BLOCKS, shared_block = b - GN;  // >= 0: one of them
+  const bool on = lane < n && (!P.live || __ldcg(P.live + lane) != 0);
+  const unsigned live = __ballot_sync(0xffffffffu, on);
+  const int nlive = __popc(live), halves = nlive > TOK ? 2 : 1;
+  const int GN = G - halves * SHARED_BLOCKS, shared_block = b - GN;  // >= 0: one of the shared expert's blocks
 
   // ---------------- the weights' stream
   Loader ld;
   ld.mode = OVER;
-  int nslot = 0, slot = 0;  // ring positions: next to fill, next to use
-  auto point = [&](const void* w, const void* s, bool int8, int row_bytes, int row0, int gap_rows, int off, int srow_bytes, int soff, int nsub, int rows_on) {
-    ld.int8 = int8;
+  uint32_t slot = ring;  // the next step's place
+  auto point = [&](const void* w, const void* s, bool int8, int row_bytes, int row0, int gap_rows, int off, int srow_bytes, int soff, int rows_on) {
     ld.stride = 4 * row_bytes, ld.gap = gap_rows * row_bytes;
     const int r = lane >> 3, c = lane & 7, sr = lane & 15;
     // Piece c (16 bytes) of row r lies where reads of eight rows at once meet no bank twice: int4 rows are read 32 bytes (four
     // lanes) at a time, int8 rows 64.
     ld.at = r * 128 + 16 * (int8 ? c ^ ((r & 1) << 2) : c ^ ((r & 3) << 1));
     ld.p = static_cast<const unsigned char*>(w) + (size_t)(row0 + r) * row_bytes + off + 16 * c;
-    ld.sp = static_cast<const unsigned char*>(s) + (size_t)(row0 + (sr < 8 ? sr : sr - 8 + gap_rows)) * srow_bytes + soff;
-    ld.sub = 0, ld.nsub = nsub;
-    ld.dp = rows_on * row_bytes - 128 * nsub, ld.ds = rows_on * srow_bytes;
+    // 16 bytes of scales a row: int4 a step's; int8 the ones around the tile's, of one row or two
+    ld.sp = static_cast<const unsigned char*>(s) + (((size_t)(row0 + (sr < 8 ? sr : sr - 8 + gap_rows)) * srow_bytes + soff) & ~(size_t)15);
+    ld.sub = int8 ? 4 : 2, ld.sstep = int8 ? 0 : 16;
+    ld.dp = rows_on * row_bytes - 128 * ld.sub, ld.ds = rows_on * srow_bytes - ld.sub * ld.sstep;
   };
-  int gu0 = 0, gu1 = 0, dn0 = 0, dn1 = 0;  // this block's tiles: expert hit x GU_TILES; shared, then expert hit x DN_TILES
+  int gu0 = 0, gu1 = 0, dn0 = 0, dn1 = 0;  // this block's tiles: entry x GU_TILES; shared halves, then entry x DN_TILES
   auto aim_gu = [&]() {
     const int h = ld.u / GU_TILES;
     ld.mode = GU, ld.ustep = 4, ld.uend = min(gu1, (h + 1) * GU_TILES);
-    point(P.w.gu_q, P.w.gu_sm, false, H / 2, ctl.hit[h] * 2 * I + 8 * (ld.u % GU_TILES), I, kq * 256, H / 64 * 4, kq * 32, 2, 32);
+    point(P.w.gu_q, P.w.gu_sm, false, H / 2, (ctl.ent[h] & 255) * 2 * I + 8 * (ld.u % GU_TILES), I, kq * 256, H / 64 * 4, kq * 32, 32);
   };
   auto aim_dn = [&]() {
-    const int h = ld.u / DN_TILES - 1, row0 = 16 * (ld.u % DN_TILES);
-    ld.mode = DN, ld.ustep = CW, ld.uend = min(dn1, (h + 2) * DN_TILES);
-    if (h < 0) point(P.w.sd_q, P.w.sd_s, true, I, row0, 8, 0, I / 128 * 2, 0, 4, 16 * CW);
-    else point(P.w.d_q, P.w.d_sm, false, I / 2, ctl.hit[h] * H + row0, 8, 0, I / 64 * 4, 0, 2, 16 * CW);
+    const int h = ld.u / DN_TILES - halves, row0 = 16 * (ld.u % DN_TILES);
+    ld.mode = DN, ld.ustep = CW, ld.uend = min(dn1, (h + halves + 1) * DN_TILES);
+    if (h < 0) point(P.w.sd_q, P.w.sd_s, true, I, row0, 8, 0, I / 128 * 2, 0, 16 * CW);
+    else point(P.w.d_q, P.w.d_sm, false, I / 2, (ctl.ent[h] & 255) * H + row0, 8, 0, I / 64 * 4, 0, 16 * CW);
   };
-  auto issue = [&]() {  // requests the next step, if there is one
+  auto next_run = [&]() {  // behind the last tile of an expert
+    if (ld.mode == GU && ld.u < gu1) return aim_gu();
+    if (ld.mode == GU) ld.mode = DN, ld.u = dn0 + warp;
+    if (ld.mode == DN && ld.u < dn1) return aim_dn();
+    ld.mode = OVER;
+  };
+  auto issue = [&](uint32_t dst) {  // requests the next step, if there is one
     if (ld.mode != OVER) {
-      const uint32_t dst = smem_u32(ring + nslot * SLOT), d = dst + ld.at;
+      const uint32_t d = dst + ld.at;
+      const unsigned char* q = ld.p + ld.gap;
       cp16(d, ld.p);
       cp16(d + 512, ld.p + ld.stride);
-      cp16(d + 1024, ld.p + ld.gap);
-      cp16(d + 1536, ld.p + ld.gap + ld.stride);
-      if (lane < 16) {
-        if (ld.int8) cp4(dst + SUB + 16 * lane, ld.sp + 4 * (ld.sub >> 1));
-        else cp16(dst + SUB + 16 * lane, ld.sp + 16 * ld.sub);
-      }
-      ld.p += 128;
-      if (++ld.sub == ld.nsub) {
-        ld.sub = 0, ld.u += ld.ustep;
-        if (ld.u < ld.uend) {
-          ld.p += ld.dp, ld.sp += ld.ds;
-        } else if (ld.mode == SHARED_GU) {
-          ld.mode = OVER;
-        } else if (ld.mode == GU && ld.u < gu1) {
-          aim_gu();
-        } else {
-          if (ld.mode == GU) ld.u = dn0 + warp;
-          if (ld.u < dn1) aim_dn();
-          else ld.mode = OVER;
-        }
+      cp16(d + 1024, q);
+      cp16(d + 1536, q + ld.stride);
+      cp16(dst + SUB + 16 * (lane & 15), ld.sp);  // both halves of the warp the same
+      ld.p += 128, ld.sp += ld.sstep;
+      if (--ld.sub == 0) {
+        ld.u += ld.ustep;
+        if (ld.u < ld.uend) ld.sub = ld.sstep ? 2 : 4, ld.p += ld.dp, ld.sp += ld.ds;
+        else next_run();
       }
     }
     cp_commit();
-    if (++nslot == DEPTH) nslot = 0;
   };
-  auto next_slot = [&]() -> const unsigned char* {
-    cp_wait<DEPTH - 1>();
-    __syncwarp();
-    return ring + slot * SLOT;
+  auto prime = [&]() {  // the ring is empty and `slot` at its next place
+#pragma unroll 1
+    for (int i = 0; i < DEPTH; ++i) {
+      issue(slot);
+      slot = slot + SLOT == ring_end ? ring : slot + SLOT;
+    }
   };
-  auto used = [&]() {
-    __syncwarp();
-    issue();
-    if (++slot == DEPTH) slot = 0;
-  };
+  // ---------------- logits: token group tg (four tokens), router rows [r0, r1); thread t holds inputs 4 t .. 4 t + 3. The rows come by copies
+  // of each thread's own eight bytes into the planes, which are free so far; behind them the shared expert's weights are requested.
+  const int tgs = (n + 3) / 4, per = GN / tgs, tg = shared_block < 0 ? b / per : tgs;
+  const int r0 = tg < tgs ? E1 * (b % per) / per : 0, r1 = tg < tgs ? E1 * (b % per + 1) / per : 0;
+  {
+    const unsigned char* src = static_cast<const unsigned char*>(P.w.router) + 8 * threadIdx.x;
+    for (int r = r0; r < r1; ++r) cp8(smem_u32(planes + (r - r0) * 2 * H + 8 * threadIdx.x), src + (size_t)r * 2 * H);
+    cp_commit();
+  }
   if (shared_block >= 0) {
     ld.mode = SHARED_GU, ld.u = 0, ld.ustep = 1, ld.uend = 1;
-    point(P.w.sgu_q, P.w.sgu_s, true, H, 8 * (4 * shared_block + quad), I, kq * 512, H / 128 * 2, kq * 8, 4, 0);
-#pragma unroll 1
-    for (int i = 0; i < DEPTH; ++i) issue();
+    point(P.w.sgu_q, P.w.sgu_s, true, H, 8 * (4 * (shared_block % SHARED_BLOCKS) + quad), I, kq * 512, H / 128 * 2, kq * 8, 0);
   }
-
-  // ---------------- logits: token group tg (four tokens), router rows [r0, r1); thread t holds inputs 4 t .. 4 t + 3
-  const int tgs = (n + 3) / 4, per = G / tgs, tg = b / per;
-  const bool part_of = tg < tgs;
-  constexpr int RP = 7;  // rows a pass
-  const int r0 = part_of ? E1 * (b % per) / per : 0, r1 = part_of ? E1 * (b % per + 1) / per : 0;
-  uint2 rw[RP];
-  auto router_rows = [&](int rb) {
-#pragma unroll
-    for (int i = 0; i < RP; ++i)
-      rw[i] = rb + i < r1 ? __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(P.w.router) + (size_t)(rb + i) * H) + threadIdx.x) : make_uint2(0u, 0u);
-  };
-  router_rows(r0);
-  const bool on = lane < n && (!P.live || __ldcg(P.live + lane) != 0);
-  const unsigned live = __ballot_sync(0xffffffffu, on);
+  prime();  // empty groups in the other blocks
   float4 xs[4];
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const int r = 4 * tg + m;
-    xs[m] = part_of && ((live >> r) & 1u) ? __ldcg(reinterpret_cast<const float4*>(P.x + (size_t)r * H) + threadIdx.x) : make_float4(0.f, 0.f, 0.f, 0.f);
+    xs[m] = r < n && ((live >> r) & 1u) ? __ldcg(reinterpret_cast<const float4*>(P.x + (size_t)r * H) + threadIdx.x) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float4 nw4 = __ldcg(reinterpret_cast<const float4*>(P.w.post_norm) + threadIdx.x);
   const unsigned ep = ld_acquire(&P.ws->epoch), tag = 2u * ep + 1u;  // this call's number
-  for (int i = threadIdx.x; i < MAX_E; i += THREADS) ctl.mask[i] = 0u;
-  if (threadIdx.x == 0) {
-    ctl.abort = 0;
-    for (int i = 0; i < 16; ++i) mbar_init(&ctl.arrived[i >> 2][i & 3], 4);
+  if (threadIdx.x < MAX_E) ctl.mask[threadIdx.x] = 0u;
+  if (threadIdx.x == 0) ctl.abort = 0;
+  if (threadIdx.x < 20) (&ctl.arrived[0][0])[threadIdx.x] = 0;
+  unsigned* done = P.ws->done[ep & 1];
+  // Four sums over the warp (one for each token): lane l gets the one of token l >> 3
+  auto sums4 = [&](float v0, float v1, float v2, float v3) {
+    const bool hi = lane & 16, mid = lane & 8;
+    const float a = (hi ? v2 : v0) + __shfl_xor_sync(0xffffffffu, hi ? v0 : v2, 16);
+    const float c = (hi ? v3 : v1) + __shfl_xor_sync(0xffffffffu, hi ? v1 : v3, 16);
+    float s = (mid ? c : a) + __shfl_xor_sync(0xffffffffu, mid ? a : c, 8);
+    s += __shfl_xor_sync(0xffffffffu, s, 4);
+    s += __shfl_xor_sync(0xffffffffu, s, 2);
+    return s + __shfl_xor_sync(0xffffffffu, s, 1);
+  };
+  if (tg < tgs) {
+    float sq[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      float4& q = xs[m];
+      sq[m] = (q.x * q.x + q.y * q.y) + (q.z * q.z + q.w * q.w);
+      q = make_float4(q.x * nw4.x, q.y * nw4.y, q.z * nw4.z, q.w * nw4.w);
+    }
+    const float s = sums4(sq[0], sq[1], sq[2], sq[3]);
+    if ((lane & 7) == 0) red[4 * warp + (lane >> 3)] = s;  // [row, squares first][warp][token]
+  }
+  cp_wait<DEPTH>();  // the router's rows
+#pragma unroll 2
+  for (int r = r0; r < r1; ++r) {
+    const uint2 w = *reinterpret_cast<const uint2*>(planes + (r - r0) * 2 * H + 8 * threadIdx.x);
+    const float a0 = __uint_as_float(w.x << 16), a1 = __uint_as_float(w.x & 0xffff0000u);
+    const float a2 = __uint_as_float(w.y << 16), a3 = __uint_as_float(w.y & 0xffff0000u);
+    float v[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) v[m] = fmaf(a3, xs[m].w, fmaf(a2, xs[m].z, fmaf(a1, xs[m].y, a0 * xs[m].x)));
+    const float s = sums4(v[0], v[1], v[2], v[3]);
+    if ((lane & 7) == 0) red[64 * (r - r0 + 1) + 4 * warp + (lane >> 3)] = s;
   }
   __syncthreads();
   if (threadIdx.x == THREADS - 1 && atom_add_acq_rel(&P.ws->seen, 1u) == (unsigned)G - 1u) {  // every block has read the number
     P.ws->seen = 0u;
     P.ws->epoch = ep + 1u;
   }
-  if (b == 0 && threadIdx.x < MAX_HIT + 8) P.ws->act_done[(ep + 1) & 1][threadIdx.x] = 0u;  // the next call's counters
+  if (b == 0 && threadIdx.x < MAX_ENT + 8) P.ws->done[(ep + 1) & 1][threadIdx.x] = 0u;  // the next call's counters
   if (live == 0u) {
     cp_wait<0>();
     return;
   }
-  unsigned* act_done = P.ws->act_done[ep & 1];
-  if (part_of) {
-    for (int rb = r0; rb < r1 || rb == r0; rb += RP) {
-      if (rb != r0) router_rows(rb);
-      float v[32];
+  for (int i = threadIdx.x; i < 4 * (r1 - r0); i += THREADS) {  // router row r0 + i / 4, token i % 4 of the group
+    const int m = i & 3, row = r0 + (i >> 2), tok = 4 * tg + m;
+    float ss = 0.f, v = 0.f;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (4 * tg + m >= n) {
-#pragma unroll
-          for (int i = 0; i < RP; ++i) v[4 * i + m] = 0.f;
-          v[28 + m] = 0.f;
-          continue;
-        }
-        const float4 q = xs[m];
-        v[28 + m] = (q.x * q.x + q.y * q.y) + (q.z * q.z + q.w * q.w);
-        const float4 h = make_float4(q.x * nw4.x, q.y * nw4.y, q.z * nw4.z, q.w * nw4.w);
-#pragma unroll
-        for (int i = 0; i < RP; ++i) {
-          const float a0 = __uint_as_float(rw[i].x << 16), a1 = __uint_as_float(rw[i].x & 0xffff0000u);
-          const float a2 = __uint_as_float(rw[i].y << 16), a3 = __uint_as_float(rw[i].y & 0xffff0000u);
-          v[4 * i + m] = fmaf(a3, h.w, fmaf(a2, h.z, fmaf(a1, h.y, a0 * h.x)));
-        }
+    for (int q = 0; q < CW; ++q) ss += red[4 * q + m], v += red[64 * ((i >> 2) + 1) + 4 * q + m];
+    const float rr = rsqrtf(ss / (float)H + P.eps);
+    if ((live >> tok) & 1u) {
+      unsigned long long* dst = P.ws->logits + tok * LOGIT_STRIDE + row;
+      stack::ll_store(dst, __float_as_uint(v * rr), tag);
+      if (row == E1 - 1) {  // behind the logits: 1 / rms, and a word that evens them out, for they are polled in pairs
+        stack::ll_store(dst + 1, __float_as_uint(rr), tag);
+        if (E & 1) stack::ll_store(dst + 2, 0u, tag);
       }
-      // 32 sums over the warp: lane l ends with sum l
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int j = 0; j < o; ++j) {
-          const bool up = lane & o;
-          const float keep = up ? v[j + o] : v[j], give = up ? v[j] : v[j + o];
-          v[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-        }
-      red[warp * 33 + lane] = v[0];
-      __syncthreads();
-      if (warp == 0) {
-        float tot = 0.f;
-#pragma unroll
-        for (int q = 0; q < CW; ++q) tot += red[q * 33 + lane];
-        const int m = lane & 3, row = rb + (lane >> 2), tok = 4 * tg + m;
-        const float rr = rsqrtf(__shfl_sync(0xffffffffu, tot, 28 + m) / (float)H + P.eps);
-        if (lane < 28 && row < r1 && (live >> tok) & 1u) {
-          unsigned long long* dst = P.ws->logits + tok * LOGIT_STRIDE + row;
-          stack::ll_store(dst, __float_as_uint(tot * rr), tag);
-          if (row == E1 - 1) {  // behind the logits: 1 / rms, and a word that evens them out, for they are polled in pairs
-            stack::ll_store(dst + 1, __float_as_uint(rr), tag);
-            if (E & 1) stack::ll_store(dst + 2, 0u, tag);
-          }
-        }
-        if (lane < 4) ctl.rr_own[4 * tg + lane] = rr;
-      }
-      __syncthreads();
     }
   }
 
-  // ---------------- digit planes of the tokens in `want`: as many warps a token as there are to spare
-  auto convert_tokens = [&](unsigned want, bool squares) {
-    const int m = __popc(want), lg = m <= 1 ? 4 : m <= 2 ? 3 : m <= 4 ? 2 : m <= 8 ? 1 : 0, nth = warp >> lg, part = warp & ((1 << lg) - 1);
-    if (nth >= m) return;
-    unsigned left = want;
-    for (int i = 0; i < nth; ++i) left &= left - 1u;
-    const int tok = __ffs(left) - 1, its = 16 >> lg, k0 = part * its;
-    const float4* xp = reinterpret_cast<const float4*>(P.x + (size_t)tok * H) + 32 * k0 + lane;
-    const float4* np = reinterpret_cast<const float4*>(P.w.post_norm) + 32 * k0 + lane;
-    unsigned char* plane = planes + 3 * tok * PITCH + 128 * k0;
-    float4* mt = meta + tok * MP + 2 * k0;
-    float ss = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < its; ++i) {
-      const float4 a = __ldcg(xp + 32 * i), c = __ldcg(np + 32 * i);
-      ss += (a.x * a.x + a.y * a.y) + (a.z * a.z + a.w * a.w);
-      digits4(make_float4(a.x * c.x, a.y * c.y, a.z * c.z, a.w * c.w), plane + 128 * i, PITCH, mt + 2 * i, lane);
+  // Digits: warp w of block b turns 256 inputs of a token into them, for all blocks: eighth b + GN w of the n tokens
+  const int item = b + GN * warp, itok = item >> 3;
+  if (shared_block < 0 && item < 8 * n && ((live >> itok) & 1u)) {
+    unsigned char* dst = P.digits + (size_t)itok * TOKEN_BYTES;
+    const float4* xp = reinterpret_cast<const float4*>(P.x + (size_t)itok * H) + 64 * (item & 7) + lane;
+    const float4* np = reinterpret_cast<const float4*>(P.w.post_norm) + 64 * (item & 7) + lane;
+    const float4 x0 = __ldcg(xp), x1 = __ldcg(xp + 32), w0 = __ldcg(np), w1 = __ldcg(np + 32);
+    float4* mt = reinterpret_cast<float4*>(dst + TOKEN_PLANES) + 4 * (item & 7);
+    dst += 256 * (item & 7);
+    digits4(make_float4(x0.x * w0.x, x0.y * w0.y, x0.z * w0.z, x0.w * w0.w), dst, PITCH, mt, lane);
+    digits4(make_float4(x1.x * w1.x, x1.y * w1.y, x1.z * w1.z, x1.w * w1.w), dst + 128, PITCH, mt + 2, lane);
+    __syncwarp();
+    if (lane == 0) {
+      __threadfence();
+      atomicAdd(done + DIGITS, 1u);
     }
-    if (squares) {
-      ss = warp_sum(ss);
-      if (lane == 0) ctl.ss[warp] = ss;
+  }
+
+  // The tokens of an entry: `code` as in ctl.ent, -1, -2: the shared expert's halves
+  auto tokens = [&](int code) {
+    unsigned m = code < 0 ? live : ctl.mask[code & 255];
+    const bool second = code < 0 ? code == -2 : code > 255;
+    if (__popc(m) > TOK) {
+      unsigned rest = m;
+      for (int i = 0; i < TOK; ++i) rest &= rest - 1u;
+      m = second ? rest : m ^ rest;
     }
+    return m;
   };
-  // The tokens of expert `e` (-1: all live ones, the shared expert), by one warp
-  auto list = [&](Seg& s, int e, bool by_place, int base, const float* rr) {
-    const unsigned m = e < 0 ? live : ctl.mask[e];
-    if (lane < MAX_TOK && (m >> lane) & 1u) {
+  // They become a segment, with digit planes from `base` on; by one warp
+  auto list = [&](Seg& s, int code, int base) {
+    const unsigned m = tokens(code);
+    if ((m >> lane) & 1u) {
       const int p = __popc(m & ((1u << lane) - 1u));
       int k = 0;
-      if (e >= 0)
-        while (k + 1 < topk && ctl.idx[lane][k] != e) ++k;
-      s.pos[p] = (unsigned char)(by_place ? base + p : lane);
-      s.row[p] = (short)(e < 0 ? n * topk + lane : lane * topk + k);
-      s.wt[p] = e < 0 ? sigmoid_f(ctl.sgate[lane]) : ctl.wts[lane][k];
-      s.rr[p] = rr[lane];
+      if (code >= 0)
+        while (k + 1 < topk && ctl.idx[lane][k] != (code & 255)) ++k;
+      s.pos[p] = (unsigned char)(base + p);
+      s.row[p] = (short)(code < 0 ? n * topk + lane : lane * topk + k);
+      s.wt[p] = code < 0 ? sigmoid_f(ctl.sgate[lane]) : ctl.wts[lane][k];
+      s.rr[p] = ctl.rr[lane];
     }
     if (lane == 0) s.count = __popc(m);
   };
-
-  // A quad's gate/up tiles u, u + 4, ... < end of one expert: each warp a quarter of the inputs; the sums meet in shared memory. With one
-  // or two tokens the warps take turns at a tile's end and need not wait for one another: a warp is at most three tiles ahead of the one
-  // whose turn it is, its own turn stops it, and four buffers and barriers serve. The finished tiles are counted once for the block, at
-  // its end (a fence a tile, which also waits for the copies under way, took as long as the tile).
-  int turn = 0;
-  auto gate_up = [&](auto tg_c, auto int8_c, const Seg& s, int u, int end) {
-    constexpr int TG = decltype(tg_c)::value;
-    constexpr bool INT8 = decltype(int8_c)::value;
-    const int g = lane >> 2, t = lane & 3;
-    float* mine = red + quad * 512;
-    if (TG) quad_sync(quad);
-    Cols<TG> c;
-    cols_set<TG>(c, s, planes, PITCH, meta, MP, lane);
-#pragma unroll 1
-    for (; u < end; u += 4) {
-      Acc<TG> acc = {};
-#pragma unroll 1
-      for (int sub = 0; sub < (INT8 ? 4 : 2); ++sub) {
-        step<TG, INT8>(acc, c, PITCH, 8 * kq + (INT8 ? 2 : 4) * sub, next_slot(), sub, lane);
-        used();
-      }
-      const int tile = u % GU_TILES;
-      if constexpr (TG == 0) {
-        const float a0 = acc.v[0] + __shfl_xor_sync(0xffffffffu, acc.v[0], 1), a1 = acc.v[1] + __shfl_xor_sync(0xffffffffu, acc.v[1], 1);
-        float* buf = mine + (turn & 3) * 128;  // [quarter][16 rows][2 tokens]
-        if ((t & 1) == 0) buf[32 * kq + 2 * g + (t >> 1)] = a0, buf[32 * kq + 2 * (g + 8) + (t >> 1)] = a1;
-        uint64_t* bar = &ctl.arrived[quad][turn & 3];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-        if (kq == (turn & 3)) {
-          mbar_wait_hot(bar, (unsigned)(turn >> 2) & 1u, DRB_ERR_GRID_WAIT);
-          const int j = (lane >> 1) & 7, p = lane & 1;
-          if (lane < 16 && p < s.count) {
-            const float* gp = buf + 2 * j + p;
-            const float rr = s.rr[p];
-            const float gate = ((gp[0] + gp[32]) + (gp[64] + gp[96])) * rr, up = ((gp[16] + gp[48]) + (gp[80] + gp[112])) * rr;
-            __stcg(P.act + (size_t)s.row[p] * I + 8 * tile + j, silu_f(gate) * up);
-          }
-        }
-        ++turn;
-      } else {
-        const int th = threadIdx.x & 127;
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-          float* st = mine + 128 * kq;  // [16 rows][8 tokens]
-          *reinterpret_cast<float2*>(st + 8 * g + 2 * t) = make_float2(acc.v[4 * i], acc.v[4 * i + 1]);
-          *reinterpret_cast<float2*>(st + 8 * (g + 8) + 2 * t) = make_float2(acc.v[4 * i + 2], acc.v[4 * i + 3]);
-          quad_sync(quad);
-          const int j = th & 7, p = 8 * i + (th >> 3);  // unit of the tile, token
-          if (th < 64 && p < s.count) {
-            const float* gp = mine + 8 * j + (th >> 3);
-            const float rr = s.rr[p];
-            const float gate = ((gp[0] + gp[128]) + (gp[256] + gp[384])) * rr, up = ((gp[64] + gp[192]) + (gp[320] + gp[448])) * rr;
-            __stcg(P.act + (size_t)s.row[p] * I + 8 * tile + j, silu_f(gate) * up);
-          }
-          quad_sync(quad);
-        }
-      }
-    }
-  };
-  using std::integral_constant;
-  auto gate_up_any = [&](auto int8_c, const Seg& s, int u, int end) {
-    if (s.count <= 2) gate_up(integral_constant<int, 0>(), int8_c, s, u, end);
-    else if (TOK <= 8 || s.count <= 8) gate_up(integral_constant<int, 1>(), int8_c, s, u, end);
-    else gate_up(integral_constant<int, 2>(), int8_c, s, u, end);
-  };
-
-  const bool early = tgs == 1 || shared_block >= 0;
-  if (early) {
-    convert_tokens(live, tgs > 1);
-    if (shared_block >= 0) {
-      if (tgs > 1) {  // 1 / rms of the tokens whose logits are other blocks' work
-        __syncthreads();
-        const int m = __popc(live), lg = m <= 1 ? 4 : m <= 2 ? 3 : m <= 4 ? 2 : m <= 8 ? 1 : 0;
-        if (threadIdx.x < MAX_TOK && (live >> threadIdx.x) & 1u) {
-          const int at = __popc(live & ((1u << threadIdx.x) - 1u)) << lg;
-          float ss = 0.f;
-          for (int i = 0; i < 1 << lg; ++i) ss += ctl.ss[at + i];
-          ctl.rr_own[threadIdx.x] = rsqrtf(ss / (float)H + P.eps);
-        }
-        __syncwarp();
-      }
-      if (warp == 0) list(ctl.seg[0], -1, false, 0, ctl.rr_own);
-      __syncthreads();
-      gate_up_any(integral_constant<bool, true>(), ctl.seg[0], 4 * shared_block + quad, 4 * shared_block + quad + 1);
-    }
-  }
-
-  // ---------------- routing: a warp a token; every block for itself
-  if ((live >> warp) & 1u) {
-    const unsigned long long* src = P.ws->logits + warp * LOGIT_STRIDE;
-    const int pieces = (E + 3) / 2;
-    uint32_t v[10];
-    unsigned need = 0u;
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {
-      v[2 * i] = v[2 * i + 1] = 0u;
-      if (lane + 32 * i < pieces) need |= 1u << i;
-    }
-    for (unsigned it = 0; !*abort_flag; ++it) {  // all requests of a round go out before any is looked at
-      unsigned long long q[10];
-#pragma unroll
-      for (int i = 0; i < 5; ++i)
-        if ((need >> i) & 1u) stack::ll_load2(src + 2 * (lane + 32 * i), q[2 * i], q[2 * i + 1]);
-#pragma unroll
-      for (int i = 0; i < 5; ++i)
-        if (((need >> i) & 1u) && (uint32_t)(q[2 * i] >> 32) == tag && (uint32_t)(q[2 * i + 1] >> 32) == tag) {
-          v[2 * i] = (uint32_t)q[2 * i], v[2 * i + 1] = (uint32_t)q[2 * i + 1];
-          need &= ~(1u << i);
-        }
-      if (need == 0u || stack::poll_failed(it, P.poll_limit, abort_flag)) break;
-    }
-    __syncwarp();
-    // larger logit = larger key, never 0; 0: no entry, or taken. A NaN counts as the lowest logit
-    uint32_t key[8];
-#pragma unroll
-    for (int i = 0; i < 10; ++i) {
-      const int id = 2 * (lane + 32 * (i >> 1)) + (i & 1);
-      if (id == E) ctl.sgate[warp] = __uint_as_float(v[i]);
-      if (id == E + 1) ctl.rr[warp] = __uint_as_float(v[i]);
-      if (i < 8) {
-        const uint32_t o = (v[i] & 0x7fffffffu) > 0x7f800000u ? 1u : (v[i] & 0x80000000u) ? ~v[i] : (v[i] | 0x80000000u);
-        key[i] = id < E ? o : 0u;
-      }
-    }
-    uint32_t mykey = 0u;
-    int myid = 0;
-    for (int k = 0; k < topk; ++k) {
-      uint32_t bk[4];
-      int bi[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // ids ascend within a lane: an equal key further on does not win
-        const bool second = key[2 * i + 1] > key[2 * i];
-        bk[i] = second ? key[2 * i + 1] : key[2 * i], bi[i] = 2 * i + (second ? 1 : 0);
-      }
-      if (bk[1] > bk[0]) bk[0] = bk[1], bi[0] = bi[1];
-      if (bk[3] > bk[2]) bk[2] = bk[3], bi[2] = bi[3];
-      if (bk[2] > bk[0]) bk[0] = bk[2], bi[0] = bi[2];
-      const int id = 2 * (lane + 32 * (bi[0] >> 1)) + (bi[0] & 1);
-      const uint32_t best = __reduce_max_sync(0xffffffffu, bk[0]);
-      const unsigned tie = __ballot_sync(0xffffffffu, bk[0] == best);
-      int who;
-      if (tie & (tie - 1u)) who = (int)__reduce_min_sync(0xffffffffu, bk[0] == best ? (unsigned)id : (unsigned)MAX_E);
-      else who = __shfl_sync(0xffffffffu, id, __ffs(tie) - 1);
-      const bool winner = id == who;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (winner && bi[0] == i) key[i] = 0u;
-      if (lane == k) mykey = best, myid = who;
-    }
-    const float val = mykey == 1u ? __uint_as_float(0x7fffffffu) : __uint_as_float((mykey & 0x80000000u) ? (mykey & 0x7fffffffu) : ~mykey);
-    const float top = __shfl_sync(0xffffffffu, val, 0), ex = lane < topk ? expf(val - top) : 0.f;
-    const float sum = warp_sum(ex);
-    if (lane < topk) {
-      ctl.idx[warp][lane] = myid, ctl.wts[warp][lane] = ex / sum;
-      atomicOr(&ctl.mask[myid], 1u << warp);
-    }
-  }
-  __syncthreads();
-  // ---------------- experts hit, in ascending order, and this block's runs of their tiles: equal shares of what the tiles cost
-  {
-    const int ec = threadIdx.x < MAX_E ? __popc(ctl.mask[threadIdx.x]) : 0;
-    const unsigned any = __ballot_sync(0xffffffffu, ec > 0), mid = __ballot_sync(0xffffffffu, ec > 2), big = __ballot_sync(0xffffffffu, ec > 8);
-    if (warp < 8 && lane == 0) ctl.wsum[warp] = __popc(any) | __popc(mid) << 8 | __popc(big) << 16;
-    if (threadIdx.x < 4) ctl.range[threadIdx.x] = -1;
-    __syncthreads();
-    if (warp < 8) {
-      int base = 0, all = 0;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const int c = ctl.wsum[w];
-        base += w < warp ? c : 0;
-        all += c;
-      }
-      const unsigned below = (1u << lane) - 1u;
-      base += __popc(any & below) | __popc(mid & below) << 8 | __popc(big & below) << 16;
-      const auto cost = [](int c) { return 4 * (c & 0xff) + 2 * ((c >> 8) & 0xff) + 5 * (c >> 16); };  // tile_cost of so many experts
-      const int h = base & 0xff, nhit = all & 0xff, before = cost(base), total = cost(all);
-      if (ec > 0) ctl.hit[h] = (unsigned char)threadIdx.x;
-      if (threadIdx.x == 0) ctl.nhit = nhit;
-      // gate/up: the shared expert's blocks have done SHARED_HEAD_START tiles more, more yet with many tokens
-      const int head = SHARED_HEAD_START * tile_cost(__popc(live)), sum = GU_TILES * total;
-      const int mine = min(sum, (sum + SHARED_BLOCKS * head) / G * GN);  // what the other blocks do
-      const int c = tile_cost(ec);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int bb = b + q;
-        const int at = bb <= GN ? mine * bb / GN : mine + (sum - mine) * (bb - GN) / SHARED_BLOCKS;
-        const int off = at - GU_TILES * before;
-        if (ec > 0 && off >= 0 && off < GU_TILES * c) ctl.range[q] = h * GU_TILES + (off + c - 1) / c;
-        if (threadIdx.x == 0 && at >= sum) ctl.range[q] = nhit * GU_TILES;
-      }
-      // down: the shared expert's tiles first; twice the bytes
-      const int cs = tile_cost(__popc(live)) + 4, dsum = DN_TILES * (total + cs);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int at = (int)((long long)dsum * (b + q) / G);
-        const int off = at - DN_TILES * (cs + before);
-        if (ec > 0 && off >= 0 && off < DN_TILES * c) ctl.range[2 + q] = (h + 1) * DN_TILES + (off + c - 1) / c;
-        if (threadIdx.x == 0 && at < DN_TILES * cs) ctl.range[2 + q] = (at + cs - 1) / cs;
-        if (threadIdx.x == 0 && at >= dsum) ctl.range[2 + q] = (nhit + 1) * DN_TILES;
-      }
-    }
-    __syncthreads();
-  }
-  gu0 = ctl.range[0], gu1 = ctl.range[1], dn0 = ctl.range[2], dn1 = ctl.range[3];
-  if (gu0 + quad < gu1) {
-    ld.u = gu0 + quad;
-    aim_gu();
-  } else if (dn0 + warp < dn1) {
-    ld.u = dn0 + warp;
-    aim_dn();
-  }
-#pragma unroll 1
-  for (int i = 0; i < DEPTH; ++i) issue();
-
-  const int h0 = gu0 / GU_TILES, split = min(gu1, (h0 + 1) * GU_TILES);  // the second expert's tiles start there
-  if (gu1 > gu0) {
-    const int e0 = ctl.hit[h0], e1 = gu1 > split ? ctl.hit[h0 + 1] : e0;
-    if (warp < 2) list(ctl.seg[warp], warp ? e1 : e0, false, 0, ctl.rr);
-    if (!early) convert_tokens(ctl.mask[e0] | ctl.mask[e1], false);
-  }
-  __syncthreads();
-  if (gu1 > gu0) {
-    gate_up_any(integral_constant<bool, false>(), ctl.seg[0], gu0 + quad, split);
-    if (gu1 > split) gate_up_any(integral_constant<bool, false>(), ctl.seg[1], split + ((gu0 + quad - split) & 3), gu1);
-  }
-  __syncthreads();  // the planes are free
-  if (threadIdx.x == 0) {
-    __threadfence();
-    if (split > gu0) atomicAdd(act_done + h0, (unsigned)(split - gu0));
-    if (gu1 > split) atomicAdd(act_done + h0 + 1, (unsigned)(gu1 - split));
-    if (shared_block >= 0) atomicAdd(act_done + MAX_HIT, 4u);
-  }
-
-  // ---------------- down: digit planes of the (at most two) experts' activations; h = -1: the shared expert
-  const int d0 = dn0 / DN_TILES - 1, d1 = dn1 > dn0 ? (dn1 - 1) / DN_TILES - 1 : d0, dsplit = min(dn1, (d0 + 2) * DN_TILES);
-  if (warp < 2 && dn1 > dn0) {
-    const int h = warp == 0 ? d0 : d1;
-    list(ctl.seg[warp], h < 0 ? -1 : ctl.hit[h], true, warp * TOK, ctl.rr);
-    if (lane == 0 && !*abort_flag)
-      for (unsigned it = 0; ld_acquire(act_done + (h < 0 ? MAX_HIT : h)) < (unsigned)GU_TILES; ++it)
+  // Their digits are requested into planes from `base` on, once they are written
+  auto copy_tokens = [&](unsigned want, int base) {
+    if (want && !*abort_flag)
+      for (unsigned it = 0; ld_acquire(done + DIGITS) < 8u * nlive; ++it)
         if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
-  }
-  __syncthreads();
-  if (dn1 > dn0) {
-    const int c0 = ctl.seg[0].count, all = c0 + (d1 != d0 ? ctl.seg[1].count : 0);
-    for (int i = warp; i < 4 * all; i += CW) {  // 128 inputs of a token
-      const int a = i >> 2, part = i & 3;
-      const Seg& s = ctl.seg[a >= c0];
-      const int p = a >= c0 ? a - c0 : a, pos = s.pos[p];
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(P.act + (size_t)s.row[p] * I) + 32 * part + lane);
-      digits4(v, planes + 3 * pos * DPITCH + 128 * part, DPITCH, meta + pos * DMP + 2 * part, lane);
-    }
-  }
-  __syncthreads();
-
-  auto down = [&](auto tg_c, auto int8_c, const Seg& s, int u, int end) {
-    constexpr int TG = decltype(tg_c)::value;
-    constexpr bool INT8 = decltype(int8_c)::value;
-    Cols<TG> c;
-    cols_set<TG>(c, s, planes, DPITCH, meta, DMP, lane);
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll 1
-    for (; u < end; u += CW) {
-      Acc<TG> acc = {};
-#pragma unroll 1
-      for (int sub = 0; sub < (INT8 ? 4 : 2); ++sub) {
-        step<TG, INT8>(acc, c, DPITCH, (INT8 ? 2 : 4) * sub, next_slot(), sub, lane);
-        used();
+    const int i = threadIdx.x;
+    if (i < TOKEN_BYTES / 16)
+      for (; want; want &= want - 1u, ++base) {
+        const uint32_t dst = i < TOKEN_PLANES / 16 ? smem_u32(planes + base * TOKEN_PLANES) + 16 * i : smem_u32(meta + base * MP) + 16 * i - TOKEN_PLANES;
+        cp16(dst, P.digits + (size_t)(__ffs(want) - 1) * TOKEN_BYTES + 16 * i);
       }
-      float* out = P.part + 16 * (u % DN_TILES) + g;
-      auto put = [&](int p, float lo, float hi) {
-        if (p < s.count) {
-          float* o = out + (size_t)s.row[p] * H;
-          __stcg(o, lo * s.wt[p]);
-          __stcg(o + 8, hi * s.wt[p]);
+    cp_commit();
+  };
+
+  // ---------------- three stages with the same body: the shared expert's gate/up (its blocks only, before the routing is known), gate/up, down.
+  // Each gets its tiles' tokens as digit planes and goes through its run of tiles, of two entries at most.
+  int turn = 0;
+#pragma unroll 1
+  for (int stage = shared_block >= 0 ? 0 : 1; stage < 3; ++stage) {
+    int first = 0, split = 0, end = 0;  // tiles: [first, split) of one entry, [split, end) of the next
+    int code1 = 0;                      // the second one, whose tokens' planes follow when the first one is through
+    bool later = false;
+    if (stage == 0) {
+      const int code = -1 - shared_block / SHARED_BLOCKS;
+      if (warp == 0) {
+        if ((live >> lane) & 1u) {  // 1 / rms, behind the logits
+          uint32_t out[2];
+          stack::ll_poll<1>(P.ws->logits + lane * LOGIT_STRIDE + ((E + 1) & ~1), tag, out, P.poll_limit, abort_flag);
+          ctl.rr[lane] = __uint_as_float(out[E & 1 ? 0 : 1]);
+        }
+        __syncwarp();
+        list(ctl.seg[0], code, 0);
+      }
+      first = 4 * (shared_block % SHARED_BLOCKS), split = end = first + 4;
+      copy_tokens(tokens(code), 0);
+      cp_wait<0>();
+    } else if (stage == 1) {
+      // ---------------- routing: a warp a token; every block for itself
+      if ((live >> warp) & 1u) {
+        const unsigned long long* src = P.ws->logits + warp * LOGIT_STRIDE;
+        const int pieces = (E + 3) / 2;
+        uint32_t v[10];
+        unsigned need = 0u;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          v[2 * i] = v[2 * i + 1] = 0u;
+          if (lane + 32 * i < pieces) need |= 1u << i;
+        }
+        for (unsigned it = 0; !*abort_flag; ++it) {  // all requests of a round go out before any is looked at
+          unsigned long long q[10];
+#pragma unroll
+          for (int i = 0; i < 5; ++i)
+            if ((need >> i) & 1u) stack::ll_load2(src + 2 * (lane + 32 * i), q[2 * i], q[2 * i + 1]);
+#pragma unroll
+          for (int i = 0; i < 5; ++i)
+            if (((need >> i) & 1u) && (uint32_t)(q[2 * i] >> 32) == tag && (uint32_t)(q[2 * i + 1] >> 32) == tag) {
+              v[2 * i] = (uint32_t)q[2 * i], v[2 * i + 1] = (uint32_t)q[2 * i + 1];
+              need &= ~(1u << i);
+            }
+          if (need == 0u || stack::poll_failed(it, P.poll_limit, abort_flag)) break;
+        }
+        __syncwarp();
+        // larger logit = larger key, never 0; 0: no entry, or taken. A NaN counts as the lowest logit
+        uint32_t key[8];
+#pragma unroll
+        for (int i = 0; i < 10; ++i) {
+          const int id = 2 * (lane + 32 * (i >> 1)) + (i & 1);
+          if (id == E) ctl.sgate[warp] = __uint_as_float(v[i]);
+          if (id == E + 1) ctl.rr[warp] = __uint_as_float(v[i]);
+          if (i < 8) {
+            const uint32_t o = (v[i] & 0x7fffffffu) > 0x7f800000u ? 1u : (v[i] & 0x80000000u) ? ~v[i] : (v[i] | 0x80000000u);
+            key[i] = id < E ? o : 0u;
+          }
+        }
+        uint32_t mykey = 0u;
+        int myid = 0;
+        for (int k = 0; k < topk; ++k) {
+          uint32_t bk[4];
+          int bi[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // ids ascend within a lane: an equal key further on does not win
+            const bool second = key[2 * i + 1] > key[2 * i];
+            bk[i] = second ? key[2 * i + 1] : key[2 * i], bi[i] = 2 * i + (second ? 1 : 0);
+          }
+          if (bk[1] > bk[0]) bk[0] = bk[1], bi[0] = bi[1];
+          if (bk[3] > bk[2]) bk[2] = bk[3], bi[2] = bi[3];
+          if (bk[2] > bk[0]) bk[0] = bk[2], bi[0] = bi[2];
+          const int id = 2 * (lane + 32 * (bi[0] >> 1)) + (bi[0] & 1);
+          const uint32_t best = __reduce_max_sync(0xffffffffu, bk[0]);
+          const unsigned tie = __ballot_sync(0xffffffffu, bk[0] == best);
+          int who;
+          if (tie & (tie - 1u)) who = (int)__reduce_min_sync(0xffffffffu, bk[0] == best ? (unsigned)id : (unsigned)MAX_E);
+          else who = __shfl_sync(0xffffffffu, id, __ffs(tie) - 1);
+          const bool winner = id == who;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (winner && bi[0] == i) key[i] = 0u;
+          if (lane == k) mykey = best, myid = who;
+        }
+        const float val = mykey == 1u ? __uint_as_float(0x7fffffffu) : __uint_as_float((mykey & 0x80000000u) ? (mykey & 0x7fffffffu) : ~mykey);
+        const float top = __shfl_sync(0xffffffffu, val, 0), ex = lane < topk ? expf(val - top) : 0.f;
+        const float sum = warp_sum(ex);
+        if (lane < topk) {
+          ctl.idx[warp][lane] = myid, ctl.wts[warp][lane] = ex / sum;
+          atomicOr(&ctl.mask[myid], 1u << warp);
+        }
+      }
+      __syncthreads();
+      // ---------------- experts hit, in ascending order, and this block's runs of their tiles: equal shares of what the tiles cost
+      {
+        const int ec = threadIdx.x < MAX_E ? __popc(ctl.mask[threadIdx.x]) : 0;
+        // an entry; with more than two tokens; a second entry; with more than two tokens
+        const unsigned any = __ballot_sync(0xffffffffu, ec > 0), mid = __ballot_sync(0xffffffffu, ec > 2);
+        const unsigned two = __ballot_sync(0xffffffffu, ec > TOK), big = __ballot_sync(0xffffffffu, ec > TOK + 2);
+        if (warp < 8 && lane == 0) ctl.wsum[warp] = (__popc(any) + __popc(two)) | (__popc(mid) + __popc(big)) << 8;
+        if (threadIdx.x < 4) ctl.range[threadIdx.x] = -1;
+        __syncthreads();
+        if (warp < 8) {
+          int base = 0, all = 0;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            const int c = ctl.wsum[w];
+            base += w < warp ? c : 0;
+            all += c;
+          }
+          const unsigned below = (1u << lane) - 1u;
+          base += (__popc(any & below) + __popc(two & below)) | (__popc(mid & below) + __popc(big & below)) << 8;
+          const int h = base & 0xff, nent = all & 0xff, before = 4 * h + 2 * (base >> 8), total = 4 * nent + 2 * (all >> 8);  // tile_cost of so many
+          const int c0 = tile_cost(ec), c1 = tile_cost(ec - TOK);
+          if (ec > 0) ctl.ent[h] = (unsigned short)threadIdx.x;
+          if (ec > TOK) ctl.ent[h + 1] = (unsigned short)(threadIdx.x + 256);
+          // gate/up: the shared expert's blocks have done SHARED_HEAD_START tiles already; down: its tiles come first, with twice the bytes
+          const int lc = tile_cost(nlive), cs = lc + 4, ns = halves * SHARED_BLOCKS;
+          const int sum = GU_TILES * total, dsum = DN_TILES * (total + halves * cs), mine = min(sum, (sum + ns * SHARED_HEAD_START * lc) / G * GN);
+          // lane q < 4: border q of this block (gate/up from, to; down from, to) on the scale of costs
+          const int bb = b + (lane & 1);
+          const bool late = !(lane & 2) && bb > GN;
+          const unsigned num = lane & 2 ? dsum * bb : late ? (sum - mine) * (bb - GN) : mine * bb, den = lane & 2 ? G : late ? ns : GN;
+          const int border = (int)(num / den) + (late ? mine : 0);
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            const int at = __shfl_sync(0xffffffffu, border, q), scale = q < 2 ? GU_TILES : DN_TILES, heads = q < 2 ? 0 : halves, lead = heads * DN_TILES * cs;
+            const int off = at - lead - scale * before;
+            if (ec > 0 && off >= 0 && off < scale * c0) ctl.range[q] = (h + heads) * scale + (off + c0 - 1) / c0;
+            if (ec > TOK && off >= scale * c0 && off < scale * (c0 + c1)) ctl.range[q] = (h + heads + 1) * scale + (off - scale * c0 + c1 - 1) / c1;
+            if (threadIdx.x == 0 && at < lead) ctl.range[q] = (at + cs - 1) / cs;
+            if (threadIdx.x == 0 && at >= lead + scale * total) ctl.range[q] = (nent + heads) * scale;
+          }
+        }
+        __syncthreads();
+      }
+      gu0 = ctl.range[0], gu1 = ctl.range[1], dn0 = ctl.range[2], dn1 = ctl.range[3];
+      const int h0 = gu0 / GU_TILES;
+      first = gu0, end = gu1, split = min(gu1, (h0 + 1) * GU_TILES);
+      unsigned m0 = 0u, m1 = 0u;
+      if (first < end) {
+        m0 = tokens(ctl.ent[h0]);
+        if (split < end) m1 = tokens(code1 = ctl.ent[h0 + 1]);
+      }
+      later = __popc(m0) + __popc(m1) > TOK;
+      copy_tokens(m0, 0);
+      if (!later) copy_tokens(m1, __popc(m0));
+      else cp_commit();
+      ld.mode = GU, ld.u = gu0 + quad;
+      if (ld.u < gu1) aim_gu();
+      else next_run();
+      prime();
+      if (warp == 0 && first < end) list(ctl.seg[0], ctl.ent[h0], 0);
+      if (warp == 1 && split < end) list(ctl.seg[1], code1, later ? 0 : __popc(m0));
+      cp_wait<DEPTH>();
+    } else {
+      // the activations of this block's gate/up run are written: counted once for the block (a fence a tile, which also waits for the copies
+      // under way, took as long as the tile)
+      if (threadIdx.x == 0) {
+        const int h0 = gu0 / GU_TILES, sp = min(gu1, (h0 + 1) * GU_TILES);
+        __threadfence();
+        if (sp > gu0) atomicAdd(done + h0, (unsigned)(sp - gu0));
+        if (gu1 > sp) atomicAdd(done + h0 + 1, (unsigned)(gu1 - sp));
+        if (shared_block >= 0) atomicAdd(done + SHARED_ACT + shared_block / SHARED_BLOCKS, 4u);
+      }
+      const int h0 = dn0 / DN_TILES - halves;  // below 0: the shared expert
+      first = dn0, end = dn1, split = min(dn1, (h0 + halves + 1) * DN_TILES);
+      if (warp < 2 && (warp ? split : first) < end) {
+        const int h = h0 + warp, code = h < 0 ? -1 - (h + halves) : ctl.ent[h];
+        list(ctl.seg[warp], code, warp * TOK);
+        if (lane == 0 && !*abort_flag)
+          for (unsigned it = 0; ld_acquire(done + (h < 0 ? SHARED_ACT + h + halves : h)) < (unsigned)GU_TILES; ++it)
+            if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
+      }
+    }
+    const bool dn = stage == 2;
+    const int pitch = dn ? DPITCH : PITCH, mp = dn ? DMP : MP;
+    if (dn) __syncthreads();
+    if (dn && first < end) {  // the activations as digits: a warp takes 128 of a token at a time, two of them on the way
+      const int c0 = ctl.seg[0].count, all = 4 * (c0 + (split < end ? ctl.seg[1].count : 0));
+#pragma unroll 1
+      for (int i0 = warp; i0 < all; i0 += 2 * CW) {
+        float4 v[2];
+        int at[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = min(i0 + j * CW, all - 1), a = i >> 2;  // the last one twice, if need be
+          const Seg& s = ctl.seg[a >= c0];
+          const int p = a >= c0 ? a - c0 : a;
+          at[j] = s.pos[p] * 4 + (i & 3);
+          v[j] = __ldcg(reinterpret_cast<const float4*>(P.act + (size_t)s.row[p] * I) + 32 * (i & 3) + lane);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          digits4(v[j], planes + 3 * (at[j] >> 2) * DPITCH + 128 * (at[j] & 3), DPITCH, meta + (at[j] >> 2) * DMP + 2 * (at[j] & 3), lane);
+      }
+    }
+    __syncthreads();
+
+    const int g = lane >> 2, t = lane & 3, nw = dn ? CW : 4;  // tiles go round the warps, or round the groups of four
+    const int kg0 = dn ? 0 : 8 * kq;
+    // this lane's rows g and g + 8 in a slot (see `point`), and their scales
+    const uint32_t at4 = g * 128 + 32 * (g & 3) + 8 * t, at8 = g * 128 + 64 * (g & 1) + 16 * t, sc8 = SUB + 16 * g + 8 * ((dn ? g : kq) & 1);
+    int u = first + (dn ? warp : quad);
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+      const int stop = k ? end : split;
+      if (k == 1) {
+        if (split >= end) break;
+        if (later) {
+          __syncthreads();
+          copy_tokens(tokens(code1), 0);
+          cp_wait<0>();
+          __syncthreads();
+        }
+      }
+      const Seg& s = ctl.seg[k];
+      const bool int8 = stage == 0 || (dn && stop <= halves * DN_TILES);
+      const int tg = s.count <= 2 ? 0 : 1;
+      float* mine = red + quad * 512;
+      if (!dn && tg) quad_sync(quad);
+      Cols c;
+      if (first < end) cols_set(c, tg, s, smem_u32(planes), pitch, smem_u32(meta), mp, lane);
+      auto steps = [&](auto tg_c, auto int8_c, float(&acc)[4]) {
+        constexpr bool INT8 = decltype(int8_c)::value;
+#pragma unroll
+        for (int sub = 0; sub < (INT8 ? 4 : 2); ++sub) {
+          cp_wait<DEPTH - 1>();
+          __syncwarp();
+          step<decltype(tg_c)::value, INT8>(acc, c, pitch, kg0 + (INT8 ? 2 : 4) * sub, slot + (INT8 ? at8 : at4), slot + (INT8 ? sc8 + 2 * sub : SUB + 16 * g));
+          __syncwarp();
+          issue(slot);
+          slot = slot + SLOT == ring_end ? ring : slot + SLOT;
         }
       };
-      if constexpr (TG == 0) {
-        const float a0 = acc.v[0] + __shfl_xor_sync(0xffffffffu, acc.v[0], 1), a1 = acc.v[1] + __shfl_xor_sync(0xffffffffu, acc.v[1], 1);
-        if ((t & 1) == 0) put(t >> 1, a0, a1);
-      } else {
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-          put(8 * i + 2 * t, acc.v[4 * i], acc.v[4 * i + 2]);
-          put(8 * i + 2 * t + 1, acc.v[4 * i + 1], acc.v[4 * i + 3]);
+      using std::integral_constant;
+#pragma unroll 1
+      for (; u < stop; u += nw) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!int8) {
+          if (tg == 0) steps(integral_constant<int, 0>(), integral_constant<bool, false>(), acc);
+          else steps(integral_constant<int, 1>(), integral_constant<bool, false>(), acc);
+        } else {
+          if (tg == 0) steps(integral_constant<int, 0>(), integral_constant<bool, true>(), acc);
+          else steps(integral_constant<int, 1>(), integral_constant<bool, true>(), acc);
+        }
+        if (tg == 0) {  // the third digit's lanes join the first two's: rows g, g + 8 of token t >> 1
+          acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 1);
+          acc[1] += __shfl_xor_sync(0xffffffffu, acc[1], 1);
+        }
+        if (dn) {
+          // 16 output rows of every token, weighted
+          auto put = [&](int p, float lo, float hi) {
+            if (p < s.count) {
+              float* o = P.part + (size_t)s.row[p] * H + 16 * (u % DN_TILES) + g;
+              __stcg(o, lo * s.wt[p]);
+              __stcg(o + 8, hi * s.wt[p]);
+            }
+          };
+          if (tg == 0) {
+            if ((t & 1) == 0) put(t >> 1, acc[0], acc[1]);
+          } else {
+            put(2 * t, acc[0], acc[2]);
+            put(2 * t + 1, acc[1], acc[3]);
+          }
+          continue;
+        }
+        // gate/up: each of the four warps holds the sums over a quarter of the inputs
+        float* act = P.act + 8 * (u % GU_TILES);
+        if (tg == 0) {
+          // The last of the four to arrive finishes the tile; the others go on, three tiles ahead of the last finished one at most, for there
+          // are four buffers.
+          float* buf = mine + (turn & 3) * 128;  // [quarter][16 rows][2 tokens]
+          for (unsigned it = 0; turn - *static_cast<volatile int*>(&ctl.finished[quad]) > 3; ++it)
+            if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
+          __syncwarp();
+          if ((t & 1) == 0) buf[32 * kq + 2 * g + (t >> 1)] = acc[0], buf[32 * kq + 2 * (g + 8) + (t >> 1)] = acc[1];
+          __syncwarp();
+          int before = 0;
+          if (lane == 0) {
+            __threadfence_block();
+            before = atomicAdd(&ctl.arrived[quad][turn & 3], 1);
+            __threadfence_block();
+          }
+          ++turn;
+          if ((__shfl_sync(0xffffffffu, before, 0) & 3) == 3) {
+            const int j = (lane >> 1) & 7, p = lane & 1;
+            if (lane < 16 && p < s.count) {
+              const float* gp = buf + 2 * j + p;
+              const float rr = s.rr[p];
+              const float gate = ((gp[0] + gp[32]) + (gp[64] + gp[96])) * rr, up = ((gp[16] + gp[48]) + (gp[80] + gp[112])) * rr;
+              __stcg(act + (size_t)s.row[p] * I + j, silu_f(gate) * up);
+            }
+            __syncwarp();
+            if (lane == 0) *static_cast<volatile int*>(&ctl.finished[quad]) = turn;
+          }
+        } else {
+          const int th = threadIdx.x & 127, j = th & 7, p = th >> 3;  // unit of the tile, token
+          float* st = mine + 128 * kq;                               // [16 rows][8 tokens]
+          *reinterpret_cast<float2*>(st + 8 * g + 2 * t) = make_float2(acc[0], acc[1]);
+          *reinterpret_cast<float2*>(st + 8 * (g + 8) + 2 * t) = make_float2(acc[2], acc[3]);
+          quad_sync(quad);
+          if (p < s.count) {
+            const float* gp = mine + 8 * j + p;
+            const float rr = s.rr[p];
+            const float gate = ((gp[0] + gp[128]) + (gp[256] + gp[384])) * rr, up = ((gp[64] + gp[192]) + (gp[320] + gp[448])) * rr;
+            __stcg(act + (size_t)s.row[p] * I + j, silu_f(gate) * up);
+          }
+          quad_sync(quad);
         }
       }
     }
-  };
-  auto down_any = [&](auto int8_c, const Seg& s, int u, int end) {
-    if (s.count <= 2) down(integral_constant<int, 0>(), int8_c, s, u, end);
-    else if (TOK <= 8 || s.count <= 8) down(integral_constant<int, 1>(), int8_c, s, u, end);
-    else down(integral_constant<int, 2>(), int8_c, s, u, end);
-  };
-  if (dn1 > dn0) {
-    int u = dn0 + warp;
-    if (d0 < 0) down_any(integral_constant<bool, true>(), ctl.seg[0], u, dsplit);
-    else down_any(integral_constant<bool, false>(), ctl.seg[0], u, dsplit);
-    if (u < dsplit) u += (dsplit - u + CW - 1) / CW * CW;
-    if (dn1 > dsplit) down_any(integral_constant<bool, false>(), ctl.seg[1], u, dn1);
+    __syncthreads();  // the planes are free, and what the stage wrote may be counted
   }
   cp_wait<0>();
 
   // ---------------- combine: once every block has written its results, each adds up its share of the outputs, in rank order
-  __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    atomicAdd(act_done + MAX_HIT + 1, 1u);
+    atomicAdd(done + BLOCKS, 1u);
     if (!*abort_flag)
-      for (unsigned it = 0; ld_acquire(act_done + MAX_HIT + 1) < (unsigned)G; ++it)
+      for (unsigned it = 0; ld_acquire(done + BLOCKS) < (unsigned)G; ++it)
         if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
   }
   __syncthreads();
@@ -828,14 +819,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
   }
 }
 
-static size_t workspace_bytes(int n, int topk) { return sizeof(Head) + (size_t)n * (topk + 1) * (I + H) * sizeof(float); }
+static size_t workspace_bytes(int n, int topk) { return sizeof(Head) + (size_t)n * ((topk + 1) * (I + H) * sizeof(float) + TOKEN_BYTES); }
 
 static cudaError_t configure_all() {
-  cudaError_t e;
-  if ((e = cudaFuncSetAttribute(k_moe_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<8>::BYTES)) != cudaSuccess) return e;
-  if ((e = cudaFuncSetAttribute(k_moe_few<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<16>::BYTES)) != cudaSuccess) return e;
-  if ((e = drb_carveout(k_moe_few<8>)) != cudaSuccess) return e;
-  return drb_carveout(k_moe_few<16>);
+  const cudaError_t e = cudaFuncSetAttribute(k_moe_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+  return e != cudaSuccess ? e : drb_carveout(k_moe_few);
 }
 
 }  // namespace few
@@ -864,10 +852,9 @@ extern "C" int drb_moe_few(const drb_moe_layer* w, const float* x, float* y, con
   p.ws = static_cast<few::Head*>(workspace);
   p.act = reinterpret_cast<float*>(p.ws + 1);
   p.part = p.act + (size_t)n * (topk + 1) * few::I;
+  p.digits = reinterpret_cast<unsigned char*>(p.part + (size_t)n * (topk + 1) * few::H);
   p.n = n, p.e = e, p.topk = topk, p.eps = eps, p.poll_limit = stack::POLL_LIMIT;
   void* args[] = {&p};
-  const bool small = n <= 8;
-  const cudaError_t err = cudaLaunchCooperativeKernel(small ? (const void*)few::k_moe_few<8> : (const void*)few::k_moe_few<16>, dim3(dev.sms),
-                                                      dim3(few::THREADS), args, small ? few::Shape<8>::BYTES : few::Shape<16>::BYTES, st);
+  const cudaError_t err = cudaLaunchCooperativeKernel((const void*)few::k_moe_few, dim3(dev.sms), dim3(few::THREADS), args, few::SMEM_BYTES, st);
   return err == cudaSuccess ? 0 : (int)err;
 }

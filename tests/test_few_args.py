@@ -49,7 +49,7 @@ def test_few_refuses_missing_and_misaligned_weights():
 def test_few_workspace_sizes():
     ws = ffi.lib().drb_moe_few_workspace_bytes
     assert ws(0, 8) == -1 and ws(17, 8) == -1 and ws(1, 0) == -1 and ws(1, 9) == -1
-    assert ws(16, 8) - ws(15, 8) == 9 * (2048 + 512) * 4 and ws(1, 1) > 0
+    assert ws(16, 8) - ws(15, 8) >= 9 * (2048 + 512) * 4 and ws(1, 1) > 0
 
 
 def lora(w=A, s=A, x=A, x_type=1, a=A, b=A, scale=A, who=A, adapters=2, rank=8, res=A, y=A, v=A, rows=4, n=64, k=512):
