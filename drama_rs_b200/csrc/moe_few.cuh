@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
     if ((lane & 7) == 0) red[4 * warp + (lane >> 3)] = s;  // [row, squares first][warp][token]
   }
   cp_wait<DEPTH>();  // the router's rows
-#pragma unroll 2
+#pragma unroll 4
   for (int r = r0; r < r1; ++r) {
     const uint2 w = *reinterpret_cast<const uint2*>(planes + (r - r0) * 2 * H + 8 * threadIdx.x);
     const float a0 = __uint_as_float(w.x << 16), a1 = __uint_as_float(w.x & 0xffff0000u);
@@ -461,11 +461,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
     }
     if (lane == 0) s.count = __popc(m);
   };
-  // Their digits are requested into planes from `base` on, once they are written
-  auto copy_tokens = [&](unsigned want, int base) {
-    if (want && !*abort_flag)
-      for (unsigned it = 0; ld_acquire(done + DIGITS) < 8u * nlive; ++it)
+  auto await = [&](int counter, unsigned count) {
+    if (!*abort_flag)
+      for (unsigned it = 0; ld_acquire(done + counter) < count; ++it)
         if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
+  };
+  // Their digits (which are written) are requested into planes from `base` on
+  auto copy_tokens = [&](unsigned want, int base) {
     const int i = threadIdx.x;
     if (i < TOKEN_BYTES / 16)
       for (; want; want &= want - 1u, ++base) {
@@ -495,9 +497,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
         list(ctl.seg[0], code, 0);
       }
       first = 4 * (shared_block % SHARED_BLOCKS), split = end = first + 4;
+      if (threadIdx.x == THREADS - 1) await(DIGITS, 8 * nlive);
+      __syncthreads();
       copy_tokens(tokens(code), 0);
       cp_wait<0>();
     } else if (stage == 1) {
+      if (threadIdx.x == THREADS - 1) await(DIGITS, 8 * nlive);  // for the copies below
       // ---------------- routing: a warp a token; every block for itself
       if ((live >> warp) & 1u) {
         const unsigned long long* src = P.ws->logits + warp * LOGIT_STRIDE;
@@ -523,8 +528,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
           if (need == 0u || stack::poll_failed(it, P.poll_limit, abort_flag)) break;
         }
         __syncwarp();
-        // larger logit = larger key, never 0; 0: no entry, or taken. A NaN counts as the lowest logit
-        uint32_t key[8];
+        // Larger logit = larger key, never 0; 0: no entry. A NaN counts as the lowest logit.
+        uint32_t key[8], low = 0u;
 #pragma unroll
         for (int i = 0; i < 10; ++i) {
           const int id = 2 * (lane + 32 * (i >> 1)) + (i & 1);
@@ -533,33 +538,39 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
           if (i < 8) {
             const uint32_t o = (v[i] & 0x7fffffffu) > 0x7f800000u ? 1u : (v[i] & 0x80000000u) ? ~v[i] : (v[i] | 0x80000000u);
             key[i] = id < E ? o : 0u;
+            low = max(low, key[i]);
           }
         }
-        uint32_t mykey = 0u;
-        int myid = 0;
-        for (int k = 0; k < topk; ++k) {
-          uint32_t bk[4];
-          int bi[4];
+        // The smallest of eight groups' maxima (four lanes each) bounds the k-th largest from below, k <= 8. The entries from it on, two or three
+        // dozen of 256, go to a list (in the planes, which are free), and everyone's rank in it is counted.
+        low = max(low, __shfl_xor_sync(0xffffffffu, low, 1));
+        low = max(low, __shfl_xor_sync(0xffffffffu, low, 2));
+        low = max(__reduce_min_sync(0xffffffffu, low), 1u);
+        uint2* cand = reinterpret_cast<uint2*>(planes) + MAX_E * warp;
+        int count = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {  // ids ascend within a lane: an equal key further on does not win
-            const bool second = key[2 * i + 1] > key[2 * i];
-            bk[i] = second ? key[2 * i + 1] : key[2 * i], bi[i] = 2 * i + (second ? 1 : 0);
-          }
-          if (bk[1] > bk[0]) bk[0] = bk[1], bi[0] = bi[1];
-          if (bk[3] > bk[2]) bk[2] = bk[3], bi[2] = bi[3];
-          if (bk[2] > bk[0]) bk[0] = bk[2], bi[0] = bi[2];
-          const int id = 2 * (lane + 32 * (bi[0] >> 1)) + (bi[0] & 1);
-          const uint32_t best = __reduce_max_sync(0xffffffffu, bk[0]);
-          const unsigned tie = __ballot_sync(0xffffffffu, bk[0] == best);
-          int who;
-          if (tie & (tie - 1u)) who = (int)__reduce_min_sync(0xffffffffu, bk[0] == best ? (unsigned)id : (unsigned)MAX_E);
-          else who = __shfl_sync(0xffffffffu, id, __ffs(tie) - 1);
-          const bool winner = id == who;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (winner && bi[0] == i) key[i] = 0u;
-          if (lane == k) mykey = best, myid = who;
+        for (int i = 0; i < 8; ++i) {
+          const bool in = key[i] >= low;
+          const unsigned bal = __ballot_sync(0xffffffffu, in);
+          if (in) cand[count + __popc(bal & ((1u << lane) - 1u))] = make_uint2(key[i], 2 * (lane + 32 * (i >> 1)) + (i & 1));
+          count += __popc(bal);
         }
+        __syncwarp();
+        uint2* best = reinterpret_cast<uint2*>(planes + CW * MAX_E * 8) + MAX_K * warp;
+        for (int c = lane; c < count; c += 32) {
+          const uint2 me = cand[c];
+          int rank = 0;
+#pragma unroll 4
+          for (int j = 0; j < count; ++j) {
+            const uint2 o = cand[j];
+            rank += o.x > me.x || (o.x == me.x && o.y < me.y) ? 1 : 0;
+          }
+          if (rank < topk) best[rank] = me;
+        }
+        __syncwarp();
+        const uint2 won = best[lane & (MAX_K - 1)];
+        const uint32_t mykey = won.x;
+        const int myid = (int)won.y;
         const float val = mykey == 1u ? __uint_as_float(0x7fffffffu) : __uint_as_float((mykey & 0x80000000u) ? (mykey & 0x7fffffffu) : ~mykey);
         const float top = __shfl_sync(0xffffffffu, val, 0), ex = lane < topk ? expf(val - top) : 0.f;
         const float sum = warp_sum(ex);
@@ -604,8 +615,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
           for (int q = 0; q < 4; ++q) {
             const int at = __shfl_sync(0xffffffffu, border, q), scale = q < 2 ? GU_TILES : DN_TILES, heads = q < 2 ? 0 : halves, lead = heads * DN_TILES * cs;
             const int off = at - lead - scale * before;
-            if (ec > 0 && off >= 0 && off < scale * c0) ctl.range[q] = (h + heads) * scale + (off + c0 - 1) / c0;
-            if (ec > TOK && off >= scale * c0 && off < scale * (c0 + c1)) ctl.range[q] = (h + heads + 1) * scale + (off - scale * c0 + c1 - 1) / c1;
+            const int round = q < 2 ? 4 : 1;  // a round of the four groups of warps
+            if (ec > 0 && off >= 0 && off < scale * c0) ctl.range[q] = (h + heads) * scale + (off + round * c0 - 1) / (round * c0) * round;
+            if (ec > TOK && off >= scale * c0 && off < scale * (c0 + c1))
+              ctl.range[q] = (h + heads + 1) * scale + (off - scale * c0 + round * c1 - 1) / (round * c1) * round;
             if (threadIdx.x == 0 && at < lead) ctl.range[q] = (at + cs - 1) / cs;
             if (threadIdx.x == 0 && at >= lead + scale * total) ctl.range[q] = (nent + heads) * scale;
           }
@@ -621,16 +634,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
         if (split < end) m1 = tokens(code1 = ctl.ent[h0 + 1]);
       }
       later = __popc(m0) + __popc(m1) > TOK;
-      copy_tokens(m0, 0);
-      if (!later) copy_tokens(m1, __popc(m0));
-      else cp_commit();
       ld.mode = GU, ld.u = gu0 + quad;
       if (ld.u < gu1) aim_gu();
       else next_run();
       prime();
+      copy_tokens(m0, 0);
+      if (!later) copy_tokens(m1, __popc(m0));
       if (warp == 0 && first < end) list(ctl.seg[0], ctl.ent[h0], 0);
       if (warp == 1 && split < end) list(ctl.seg[1], code1, later ? 0 : __popc(m0));
-      cp_wait<DEPTH>();
+      cp_wait<0>();
     } else {
       // the activations of this block's gate/up run are written: counted once for the block (a fence a tile, which also waits for the copies
       // under way, took as long as the tile)
@@ -646,9 +658,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
       if (warp < 2 && (warp ? split : first) < end) {
         const int h = h0 + warp, code = h < 0 ? -1 - (h + halves) : ctl.ent[h];
         list(ctl.seg[warp], code, warp * TOK);
-        if (lane == 0 && !*abort_flag)
-          for (unsigned it = 0; ld_acquire(done + (h < 0 ? SHARED_ACT + h + halves : h)) < (unsigned)GU_TILES; ++it)
-            if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
+        if (lane == 0) await(h < 0 ? SHARED_ACT + h + halves : h, GU_TILES);
       }
     }
     const bool dn = stage == 2;
@@ -796,9 +806,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
   if (threadIdx.x == 0) {
     __threadfence();
     atomicAdd(done + BLOCKS, 1u);
-    if (!*abort_flag)
-      for (unsigned it = 0; ld_acquire(done + BLOCKS) < (unsigned)G; ++it)
-        if (stack::poll_failed(it, P.poll_limit, abort_flag)) break;
+    await(BLOCKS, G);
   }
   __syncthreads();
   const int outs = n * H / 4, o0 = outs / G * b + min(outs % G, b), o1 = outs / G * (b + 1) + min(outs % G, b + 1);  // in fours
