@@ -2,15 +2,17 @@
 //
 //   y_r = W x_r (+ res_r) + scale_a B_a (A_a x_r),  a = adapter_of[r]
 //
-// Two launches (one without adapters). k_shrink: v_r = scale_a A_a x_r, the adapters' first halves, read once per row that uses them.
-// k_proj: the weights' stream. Bound by the bytes of W and of the adapters hit for few rows; from some 64 rows on by mma.sync.
+// Two launches (one without adapters). v_r = scale_a A_a x_r: k_shrink, a warp a dot product, or k_shrink_rows, sixteen rows a block on the
+// tensor cores. Then k_proj: the weights' stream, with the adapters' second half on its sums. Bound by the bytes of W and of the
+// adapters hit for few rows; from some 64 rows on by mma.sync.
 //
 // k_proj: 16-bit x meets the int8 codes, which both 16-bit types hold exactly, on mma.sync m16n8k16; a sum over the 128 inputs of a weight
-// scale is fp32, scaled in fp32, so no weight is rounded. The 16 weight rows of a tile are M, the rows of x are N (8 to 64 a pass). A
-// block keeps its slice of x in shared memory. 64 rows of 2048 inputs would not fit and would cost every multiprocessor 256 KB of L2
-// reads, so a cluster of blocks shares the K axis: each holds its slice of x, streams its slice of the cluster's weight rows through
-// rings of 16-byte asynchronous copies (one ring a warp, no barrier in a step), and the slices' sums meet through distributed shared
-// memory, in rank order.
+// scale is fp32, scaled in fp32, so no weight is rounded. The 16 weight rows of a tile are M, the rows of x are N (8 to 32 a pass). A
+// block keeps its slice of x in shared memory. 32 rows of 2048 inputs would cost every multiprocessor 128 KB of L2 reads, so a cluster
+// of blocks shares the K axis: each holds its slice of x, streams its slice of the cluster's weight rows through rings of 16-byte
+// asynchronous copies (one ring a warp, no barrier in a step), and the slices' sums meet through distributed shared memory, in rank
+// order. The weights' first steps are requested before the launch before has ended, and x is read and multiplied while k_shrink still
+// runs: k_shrink lets this kernel in behind its own wait, so what came before k_shrink is complete.
 #pragma once
 
 #include "common.cuh"
@@ -21,8 +23,11 @@ namespace pl {
 constexpr int MAX_RANK = 64, MAX_K = 8192;
 constexpr int CW = 8, THREADS = CW * 32;
 constexpr int SUB = 2048;                  // a step of a warp: 16 weight rows x 128 inputs
+constexpr int DEPTH = 3;
 constexpr int PP = 20;                     // floats between the columns of a tile of sums: writes of a warp meet no bank twice
-constexpr size_t SMEM_MAX = 232448;
+constexpr size_t SMEM_MAX = 232448, SMEM_TWO = 112 * 1024;  // up to the second, two blocks share a multiprocessor
+constexpr int TILE_ROWS = 64;              // more rows than these: k_shrink_rows
+constexpr int TENSOR_ADAPTERS = 4;         // adapters in a pass up to which their second half runs on the tensor cores
 
 struct Args {
   const int8_t* w;
@@ -36,34 +41,43 @@ struct Args {
 };
 
 DRB_DEV float widen16(uint32_t b, bool f16) { return f16 ? __half2float(__ushort_as_half((uint16_t)b)) : __uint_as_float(b << 16); }
+DRB_DEV int adapter(const Args& p, int row) {  // -1: none
+  const int a = __ldcg(p.adapter_of + row);
+  return a >= 0 && a < p.adapters ? a : -1;
+}
 
 // ---- v = scale A x ------------------------------------------------------------------------------------------------------
 // A block: eight ranks of one row, a warp each.
 template <bool F16>
 __global__ void __launch_bounds__(256) k_shrink(Args p) {
   const int row = (int)blockIdx.x, j = (int)blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  pdl_launch_dependents();
   pdl_wait();
-  const int ad = __ldcg(p.adapter_of + row);
-  if (ad < 0 || ad >= p.adapters) return;
-  const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (size_t)row * p.k) + lane;
-  const uint4* ap = reinterpret_cast<const uint4*>(p.a + ((size_t)ad * p.rank + j) * p.k) + lane;
+  pdl_launch_dependents();  // behind the wait: see above
+  const int ad = adapter(p, row);
+  if (ad < 0) return;
+  const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (size_t)row * p.k);
+  const uint4* ap = reinterpret_cast<const uint4*>(p.a + ((size_t)ad * p.rank + j) * p.k);
   float acc[2] = {0.f, 0.f};
-#pragma unroll 4
-  for (int i = lane; i < p.k / 8; i += 32, xp += 32, ap += 32) {
-    const uint4 xv = __ldcg(xp), av = __ldg(ap);
-    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, aw[4] = {av.x, av.y, av.z, av.w};
+  for (int i0 = lane; i0 < p.k / 8; i0 += 8 * 32) {  // eight pieces of either at once
+    uint4 xv[8], av[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      acc[0] = fmaf(widen16(xw[q] & 0xffffu, F16), widen16(aw[q] & 0xffffu, false), acc[0]);
-      acc[1] = fmaf(widen16(xw[q] >> 16, F16), widen16(aw[q] >> 16, false), acc[1]);
+    for (int q = 0; q < 8; ++q)
+      if (i0 + 32 * q < p.k / 8) xv[q] = __ldcg(xp + i0 + 32 * q), av[q] = __ldcg(ap + i0 + 32 * q);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (i0 + 32 * q >= p.k / 8) break;
+      const uint32_t xw[4] = {xv[q].x, xv[q].y, xv[q].z, xv[q].w}, aw[4] = {av[q].x, av[q].y, av[q].z, av[q].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[0] = fmaf(widen16(xw[e] & 0xffffu, F16), widen16(aw[e] & 0xffffu, false), acc[0]);
+        acc[1] = fmaf(widen16(xw[e] >> 16, F16), widen16(aw[e] >> 16, false), acc[1]);
+      }
     }
   }
   const float sum = warp_sum(acc[0] + acc[1]);
   if (lane == 0) p.v[(size_t)row * p.rank + j] = sum * __ldcg(p.scale + ad);
 }
 
-// ---- y = W x + res + B v -----------------------------------------------------------------------------------------------
 template <bool F16>
 DRB_DEV void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (F16)
@@ -96,6 +110,68 @@ DRB_DEV void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
   }
 }
 
+// Two f16 numbers as the sum of two pairs of bf16 numbers, exactly (eleven bits; eight and the rest).
+DRB_DEV void split_f16(uint32_t h, uint32_t& hi, uint32_t& lo) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  const __nv_bfloat162 a = __floats2bfloat162_rn(f.x, f.y);
+  const __nv_bfloat162 b = __floats2bfloat162_rn(f.x - __low2float(a), f.y - __high2float(a));
+  hi = *reinterpret_cast<const uint32_t*>(&a), lo = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// A block: eight ranks of sixteen rows, every adapter among them in turn; each of the eight warps an eighth of the inputs, in pieces of 32.
+// Rows are M, ranks are N; both operands straight from L2. fp16 rows meet the bf16 adapters as two bf16 terms.
+template <bool F16>
+__global__ void __launch_bounds__(256) k_shrink_rows(Args p) {
+  __shared__ int who[16];
+  __shared__ float part[8][16][8];
+  const int row0 = (int)blockIdx.x * 16, j0 = (int)blockIdx.y * 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rows = min(16, p.rows - row0);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (threadIdx.x < 16) who[threadIdx.x] = (int)threadIdx.x < rows ? adapter(p, row0 + threadIdx.x) : -1;
+  __syncthreads();
+  const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(g, rows - 1)) * p.k + 8 * t;
+  const uint16_t* x1 = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(g + 8, rows - 1)) * p.k + 8 * t;
+  const int steps = p.k / 32, c0 = steps * warp / 8, c1 = steps * (warp + 1) / 8;
+  for (int r = 0; r < rows; ++r) {
+    const int ad = who[r];
+    bool seen = ad < 0;
+    for (int q = 0; q < r; ++q) seen |= who[q] == ad;
+    if (seen) continue;  // the same in every thread
+    const uint16_t* ap = reinterpret_cast<const uint16_t*>(p.a) + ((size_t)ad * p.rank + j0 + g) * p.k + 8 * t;
+    float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int c = c0; c < c1; ++c) {
+      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(x0 + 32 * c)), v = __ldcg(reinterpret_cast<const uint4*>(x1 + 32 * c));
+      const uint4 b = __ldcg(reinterpret_cast<const uint4*>(ap + 32 * c));
+      if constexpr (F16) {
+        uint32_t uh[4], ul[4], vh[4], vl[4];
+        split_f16(u.x, uh[0], ul[0]), split_f16(u.y, uh[1], ul[1]), split_f16(u.z, uh[2], ul[2]), split_f16(u.w, uh[3], ul[3]);
+        split_f16(v.x, vh[0], vl[0]), split_f16(v.y, vh[1], vl[1]), split_f16(v.z, vh[2], vl[2]), split_f16(v.w, vh[3], vl[3]);
+        mma16<false>(d, uh[0], vh[0], uh[1], vh[1], b.x, b.y);
+        mma16<false>(e, uh[2], vh[2], uh[3], vh[3], b.z, b.w);
+        mma16<false>(d, ul[0], vl[0], ul[1], vl[1], b.x, b.y);
+        mma16<false>(e, ul[2], vl[2], ul[3], vl[3], b.z, b.w);
+      } else {
+        mma16<false>(d, u.x, v.x, u.y, v.y, b.x, b.y);
+        mma16<false>(e, u.z, v.z, u.w, v.w, b.z, b.w);
+      }
+    }
+    *reinterpret_cast<float2*>(&part[warp][g][2 * t]) = make_float2(d[0] + e[0], d[1] + e[1]);
+    *reinterpret_cast<float2*>(&part[warp][g + 8][2 * t]) = make_float2(d[2] + e[2], d[3] + e[3]);
+    __syncthreads();
+    const int m = (int)threadIdx.x >> 3, j = threadIdx.x & 7;
+    if (m < rows && who[m] == ad) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s += part[q][m][j];
+      p.v[(size_t)(row0 + m) * p.rank + j0 + j] = s * __ldcg(p.scale + ad);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- y = W x + res + B v -----------------------------------------------------------------------------------------------
 DRB_DEV unsigned cluster_size() {
   unsigned v;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(v));
@@ -108,51 +184,76 @@ DRB_DEV unsigned cluster_rank() {
 }
 DRB_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 DRB_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-DRB_DEV float ld_peer(uint32_t addr, unsigned rank) {
+DRB_DEV float4 ld_peer(uint32_t addr, unsigned rank) {
   uint32_t a;
-  float v;
+  float4 v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
 
+// NT column tiles (8 rows of x each) a pass; a slice of K inputs.
 template <int NT>
 struct Shape {
-  static constexpr int DEPTH = NT == 8 ? 3 : 6;
-  static constexpr size_t SUMS = (size_t)CW * 8 * NT * PP * 4;
-  static constexpr size_t bytes(int slice) { return (size_t)8 * NT * (2 * slice + 16) + SUMS + (size_t)CW * DEPTH * SUB; }
+  static constexpr size_t SUMS = (size_t)CW * 8 * NT * PP * 4, RING = (size_t)CW * DEPTH * SUB;
+  static constexpr size_t VS = (size_t)8 * NT * (MAX_RANK + 4) * 4;  // v of the pass, where the tensor cores take it
+  static constexpr size_t bytes(int slice) { return 256 + (size_t)8 * NT * (2 * slice + 16) + SUMS + RING + VS; }
 };
-static_assert(Shape<8>::bytes(MAX_K / 8) <= SMEM_MAX && Shape<4>::bytes(MAX_K / 8) <= SMEM_MAX, "eight blocks hold the longest row");
+static_assert(Shape<4>::bytes(MAX_K / 8) <= SMEM_MAX, "eight blocks hold the longest row");
 
-// NT: column tiles (8 rows of x each) of a pass; blockIdx.y: the pass. Cluster c of the pass owns weight tiles [mt c / C, mt (c + 1) / C).
+// Four fp32 numbers as pairs of bf16 numbers in three terms (eight bits each, the third rounded).
+DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
+  float4 r = v;
+#pragma unroll
+  for (int l = 0; l < 3; ++l) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(r.x, r.y), c = __floats2bfloat162_rn(r.z, r.w);
+    b0[l] = *reinterpret_cast<const uint32_t*>(&a), b1[l] = *reinterpret_cast<const uint32_t*>(&c);
+    r = make_float4(r.x - __low2float(a), r.y - __high2float(a), r.z - __low2float(c), r.w - __high2float(c));
+  }
+}
+
+// blockIdx.y: the pass of 8 NT rows of x. Cluster c of the pass owns weight tiles [mt c / C, mt (c + 1) / C), kw warps of a block share a tile.
 template <bool F16, int NT>
-__global__ void __launch_bounds__(THREADS, 1) k_proj(Args p) {
-  constexpr int DEPTH = Shape<NT>::DEPTH;
+__global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) {
   extern __shared__ __align__(128) unsigned char dyn[];
+  int* who = reinterpret_cast<int*>(dyn);  // [8 NT] adapters of the pass's rows, then the different ones among them and their number
+  unsigned char* xs = dyn + 256;
+  float* sums = reinterpret_cast<float*>(xs + (size_t)8 * NT * pitch);
+  float* vs = sums + Shape<NT>::SUMS / 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(vs) + Shape<NT>::VS + warp * DEPTH * SUB;
   const int cs = (int)cluster_size(), cr = (int)cluster_rank(), C = (int)gridDim.x / cs, c = (int)blockIdx.x / cs;
-  const int groups = p.k / 128, g0 = groups * cr / cs, ng = groups * (cr + 1) / cs - g0;  // this block's inputs
+  const int tw = CW / kw, wt = warp / kw, wk = warp % kw;                                   // tiles of a batch; this warp's tile and share of K
+  const int groups = p.k / 128, b0 = groups * cr / cs, bn = groups * (cr + 1) / cs - b0;    // this block's inputs, in 128s
+  const int g0 = bn * wk / kw, ng = bn * (wk + 1) / kw - g0;                                // this warp's, of the block's
   const int mt = (p.n + 15) / 16, t0 = (int)((long long)mt * c / C), t1 = (int)((long long)mt * (c + 1) / C);
   const int row0 = (int)blockIdx.y * 8 * NT, cols = min(8 * NT, p.rows - row0);
-  const int pitch = 2 * 128 * ((groups + cs - 1) / cs) + 16;
-  unsigned char* xs = dyn;
-  float* sums = reinterpret_cast<float*>(dyn + (size_t)8 * NT * pitch);
-  unsigned char* ring = reinterpret_cast<unsigned char*>(sums) + Shape<NT>::SUMS + warp * DEPTH * SUB;
+
   pdl_launch_dependents();
 
-  // The weights' stream: tiles t0 + warp, t0 + warp + CW, ..., ng steps each. Rows behind the last one are read as the last one.
-  const int mine = t1 - t0 > warp ? (t1 - t0 - warp + CW - 1) / CW : 0, steps = mine * ng;
-  int nslot = 0, slot = 0, ltile = t0 + warp, lg = 0, left = steps;
+  // The weights' stream: tiles t0 + wt, t0 + wt + tw, ..., ng steps each. Rows behind the last one are read as the last one.
+  const int mine = t1 - t0 > wt ? (t1 - t0 - wt + tw - 1) / tw : 0;
+  int nslot = 0, slot = 0, ltile = t0 + wt, lg = 0, left = mine * ng;
+  const uint32_t put = (lane >> 3) * 128 + 16 * ((lane & 7) ^ (((lane >> 3) & 1) << 2));
+  const int8_t* src = p.w;  // this lane's piece of the next step in row 16 ltile, and its four rows from there
+  int over[4] = {0, 0, 0, 0};
+  auto aim = [&]() {
+    src = p.w + (size_t)16 * ltile * p.k + (b0 + g0) * 128 + 16 * (lane & 7);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) over[i] = min((lane >> 3) + 4 * i, p.n - 1 - 16 * ltile) * p.k;
+  };
+  if (left > 0) aim();
   auto issue = [&]() {
     if (left > 0) {
-      const uint32_t dst = smem_u32(ring + nslot * SUB);
+      const uint32_t dst = ring + nslot * SUB + put;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = (lane >> 3) + 4 * i, q = lane & 7;
-        few::cp16(dst + r * 128 + 16 * (q ^ ((r & 1) << 2)), p.w + (size_t)min(16 * ltile + r, p.n - 1) * p.k + (g0 + lg) * 128 + 16 * q);
-      }
+      for (int i = 0; i < 4; ++i) few::cp16(dst + 512 * i, src + over[i]);
+      src += 128;
       --left;
-      if (++lg == ng) lg = 0, ltile += CW;
+      if (++lg == ng) {
+        lg = 0, ltile += tw;
+        if (left > 0) aim();
+      }
     }
     few::cp_commit();
     if (++nslot == DEPTH) nslot = 0;
@@ -160,46 +261,59 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj(Args p) {
 #pragma unroll 1
   for (int i = 0; i < DEPTH; ++i) issue();
   auto scales = [&](int tile, int grp, float& s0, float& s1) {
-    s0 = __half2float(__ldg(p.s + (size_t)min(16 * tile + g, p.n - 1) * groups + g0 + grp));
-    s1 = __half2float(__ldg(p.s + (size_t)min(16 * tile + g + 8, p.n - 1) * groups + g0 + grp));
+    s0 = __half2float(__ldg(p.s + (size_t)min(16 * tile + g, p.n - 1) * groups + b0 + g0 + grp));
+    s1 = __half2float(__ldg(p.s + (size_t)min(16 * tile + g + 8, p.n - 1) * groups + b0 + g0 + grp));
   };
   float s0 = 0.f, s1 = 0.f;
-  if (steps > 0) scales(t0 + warp, 0, s0, s1);
+  if (mine * ng > 0) scales(t0 + wt, 0, s0, s1);
 
-  pdl_wait();  // x, res, the adapters and v
+  if (p.rank == 0) pdl_wait();  // with adapters x and the rest are older than k_shrink, and only v is awaited, below
   {
-    const int pieces = ng * 16;  // of 16 bytes a row
+    const int pieces = bn * 16;  // of 16 bytes a row
     for (int i = threadIdx.x; i < 8 * NT * pieces; i += THREADS) {
       const int r = i / pieces, q = i - r * pieces;
-      few::cp16(smem_u32(xs + r * pitch + 16 * q), static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(r, cols - 1)) * p.k + g0 * 128 + 8 * q);
+      few::cp16(smem_u32(xs + r * pitch + 16 * q), static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(r, cols - 1)) * p.k + b0 * 128 + 8 * q);
     }
     few::cp_commit();
+    if (p.rank > 0 && threadIdx.x < 8 * NT) {
+      const int a = (int)threadIdx.x < cols ? adapter(p, row0 + threadIdx.x) : -1;
+      who[threadIdx.x] = a;
+    }
     few::cp_wait<0>();
     __syncthreads();
   }
+  int ndiff = 0;
+  if (p.rank > 0) {  // the different adapters, in every warp for itself
+    const int a = lane < 8 * NT ? who[lane] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, a);
+    const unsigned firsts = __ballot_sync(0xffffffffu, a >= 0 && __ffs(same) - 1 == lane);
+    ndiff = __popc(firsts);
+    if (warp == 0 && (firsts >> lane) & 1u) who[32 + __popc(firsts & ((1u << lane) - 1u))] = a;
+  }
+  const bool tensor = ndiff > 0 && ndiff <= TENSOR_ADAPTERS && p.rows > TILE_ROWS;
 
-  const int batches = (t1 - t0 + CW - 1) / CW;
-  const unsigned char* xb = xs + g * pitch + 32 * t;
+  const int batches = (t1 - t0 + tw - 1) / tw;
+  const uint32_t xb = smem_u32(xs) + g * pitch + 32 * t + 256 * g0;
   for (int bt = 0; bt < batches; ++bt) {
-    const int tile = t0 + bt * CW + warp;
+    const int tile = t0 + bt * tw + wt;
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     if (tile < t1) {
+#pragma unroll 1
       for (int q = 0; q < ng; ++q) {
         const float f0 = s0, f1 = s1;
         if (q + 1 < ng) scales(tile, q + 1, s0, s1);
-        else if (tile + CW < t1) scales(tile + CW, 0, s0, s1);
+        else if (tile + tw < t1) scales(tile + tw, 0, s0, s1);
         few::cp_wait<DEPTH - 1>();
         __syncwarp();
-        const unsigned char* r0 = ring + slot * SUB + g * 128;
+        const uint32_t r0 = ring + slot * SUB + g * 128 + 64 * (g & 1) + 16 * t;
         float d[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int at = 64 * (h ^ (g & 1)) + 16 * t;
-          const uint4 u = *reinterpret_cast<const uint4*>(r0 + at), v = *reinterpret_cast<const uint4*>(r0 + 8 * 128 + at);
+          const uint4 u = few::lds<uint4>(r0 ^ (64 * h)), v = few::lds<uint4>((r0 ^ (64 * h)) + 1024);
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {  // inputs 16 t + 8 e .. + 7 of the 64: two multiplications
@@ -210,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj(Args p) {
             widen_codes<F16>(vw[2 * e + 1], a[5], a[7]);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-              const uint4 b = *reinterpret_cast<const uint4*>(xb + (size_t)8 * i * pitch + q * 256 + h * 128 + 16 * e);
+              const uint4 b = few::lds<uint4>(xb + 8 * i * pitch + q * 256 + h * 128 + 16 * e);
               mma16<F16>(d[i], a[0], a[1], a[2], a[3], b.x, b.y);
               mma16<F16>(d[i], a[4], a[5], a[6], a[7], b.z, b.w);
             }
@@ -226,6 +340,41 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj(Args p) {
         }
       }
     }
+    if (p.rank > 0 && bt == 0) {
+      pdl_wait();  // v
+      if (tensor) {
+        for (int i = threadIdx.x; i < 8 * NT * (p.rank / 4); i += THREADS) {
+          const int r = i / (p.rank / 4), q = i % (p.rank / 4);
+          *reinterpret_cast<float4*>(vs + r * (MAX_RANK + 4) + 4 * q) =
+              r < cols && who[r] >= 0 ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        __syncthreads();
+      }
+    }
+    if (tensor && tile < t1) {
+      // B v as more inputs: sixteen ranks of an adapter at a time, dealt out over the K slices; rows of other adapters count as zeros
+      const int chunks = (p.rank + 15) / 16;
+#pragma unroll 1
+      for (int i0 = cr * kw + wk; i0 < ndiff * chunks; i0 += cs * kw) {
+        const int ad = who[32 + i0 / chunks], k0 = i0 % chunks * 16 + 4 * t;
+        uint2 u = make_uint2(0u, 0u), v = u;
+        const bool in = k0 < p.rank;
+        if (in) {
+          u = __ldcg(reinterpret_cast<const uint2*>(p.b + ((size_t)ad * p.n + min(16 * tile + g, p.n - 1)) * p.rank + k0));
+          v = __ldcg(reinterpret_cast<const uint2*>(p.b + ((size_t)ad * p.n + min(16 * tile + g + 8, p.n - 1)) * p.rank + k0));
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (in && who[8 * i + g] == ad) f = *reinterpret_cast<const float4*>(vs + (8 * i + g) * (MAX_RANK + 4) + k0);
+          uint32_t q0[3], q1[3];
+          split3(f, q0, q1);
+#pragma unroll
+          for (int l = 2; l >= 0; --l) mma16<false>(acc[i], u.x, v.x, u.y, v.y, q0[l], q1[l]);
+        }
+      }
+    }
+    __syncwarp();
     if (bt > 0) cluster_wait();  // everyone has read the batch before
     float* st = sums + warp * 8 * NT * PP;
 #pragma unroll
@@ -233,36 +382,52 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj(Args p) {
       st[(8 * i + 2 * t) * PP + g] = acc[i][0], st[(8 * i + 2 * t + 1) * PP + g] = acc[i][1];
       st[(8 * i + 2 * t) * PP + g + 8] = acc[i][2], st[(8 * i + 2 * t + 1) * PP + g + 8] = acc[i][3];
     }
+    __syncwarp();
     cluster_arrive();
     cluster_wait();
-    // Block cr of the cluster finishes its share of the batch: column r of x, weight row j of tile m.
-    const int nt = min(CW, t1 - t0 - bt * CW), outs = nt * 16 * cols;
+    // Block cr of the cluster finishes its share of the batch, four weight rows of a column (a row of x) at a time
+    const int nt = min(tw, t1 - t0 - bt * tw), outs = nt * 4 * cols;
     for (int i = outs * cr / cs + (int)threadIdx.x; i < outs * (cr + 1) / cs; i += THREADS) {
-      const int j = i & 15, m = (i >> 4) % nt, r = (i >> 4) / nt, o = 16 * (t0 + bt * CW + m) + j;
+      const int j = 4 * (i & 3), m = (i >> 2) % nt, r = (i >> 2) / nt, o = 16 * (t0 + bt * tw + m) + j, row = row0 + r;
       if (o >= p.n) continue;
-      const uint32_t at = smem_u32(sums + (m * 8 * NT + r) * PP + j);
-      float v = 0.f;
-      for (int q = 0; q < cs; ++q) v += ld_peer(at, (unsigned)q);
-      const int row = row0 + r;
-      if (p.rank > 0) {
-        const int ad = __ldcg(p.adapter_of + row);
-        if (ad >= 0 && ad < p.adapters) {
-          const uint4* bp = reinterpret_cast<const uint4*>(p.b + ((size_t)ad * p.n + o) * p.rank);
-          const float4* vp = reinterpret_cast<const float4*>(p.v + (size_t)row * p.rank);
-          float s = 0.f;
-          for (int q = 0; q < p.rank / 8; ++q) {
-            const uint4 bw = __ldg(bp + q);
-            const float4 v0 = __ldcg(vp + 2 * q), v1 = __ldcg(vp + 2 * q + 1);
-            s = fmaf(widen16(bw.x & 0xffffu, false), v0.x, s), s = fmaf(widen16(bw.x >> 16, false), v0.y, s);
-            s = fmaf(widen16(bw.y & 0xffffu, false), v0.z, s), s = fmaf(widen16(bw.y >> 16, false), v0.w, s);
-            s = fmaf(widen16(bw.z & 0xffffu, false), v1.x, s), s = fmaf(widen16(bw.z >> 16, false), v1.y, s);
-            s = fmaf(widen16(bw.w & 0xffffu, false), v1.z, s), s = fmaf(widen16(bw.w >> 16, false), v1.w, s);
+      const int ad = p.rank > 0 && !tensor ? who[r] : -1;
+      float4 f[8];
+      const uint32_t at = smem_u32(sums + (m * kw * 8 * NT + r) * PP + j);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < kw; ++k) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] = q < cs ? ld_peer(at + k * 8 * NT * PP * 4, (unsigned)q) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[0] += f[q].x, v[1] += f[q].y, v[2] += f[q].z, v[3] += f[q].w;
+      }
+      if (ad >= 0) {
+        const float4* vp = reinterpret_cast<const float4*>(p.v + (size_t)row * p.rank);
+        const uint4* bp = reinterpret_cast<const uint4*>(p.b + ((size_t)ad * p.n + o) * p.rank);
+        const int r8 = p.rank / 8;
+        for (int q = 0; q < r8; ++q) {
+          const float4 v0 = __ldcg(vp + 2 * q), v1 = __ldcg(vp + 2 * q + 1);
+          uint4 bw[4];
+#pragma unroll
+          for (int l = 0; l < 4; ++l) bw[l] = __ldcg(bp + min(l, p.n - 1 - o) * r8 + q);
+#pragma unroll
+          for (int l = 0; l < 4; ++l) {
+            v[l] = fmaf(widen16(bw[l].x & 0xffffu, false), v0.x, v[l]), v[l] = fmaf(widen16(bw[l].x >> 16, false), v0.y, v[l]);
+            v[l] = fmaf(widen16(bw[l].y & 0xffffu, false), v0.z, v[l]), v[l] = fmaf(widen16(bw[l].y >> 16, false), v0.w, v[l]);
+            v[l] = fmaf(widen16(bw[l].z & 0xffffu, false), v1.x, v[l]), v[l] = fmaf(widen16(bw[l].z >> 16, false), v1.y, v[l]);
+            v[l] = fmaf(widen16(bw[l].w & 0xffffu, false), v1.z, v[l]), v[l] = fmaf(widen16(bw[l].w >> 16, false), v1.w, v[l]);
           }
-          v += s;
         }
       }
       const size_t yo = (size_t)row * p.n + o;
-      p.y[yo] = p.res ? v + __ldcg(p.res + yo) : v;
+      if (p.n % 4 == 0 && (((uintptr_t)p.y | (uintptr_t)p.res) & 15) == 0) {
+        if (p.res) {
+          const float4 a = __ldcg(reinterpret_cast<const float4*>(p.res + yo));
+          v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+        }
+        *reinterpret_cast<float4*>(p.y + yo) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        for (int l = 0; l < 4 && o + l < p.n; ++l) p.y[yo + l] = p.res ? v[l] + __ldcg(p.res + yo + l) : v[l];
+      }
     }
     __syncwarp();
     cluster_arrive();
@@ -271,17 +436,32 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj(Args p) {
   few::cp_wait<0>();
 }
 
-// NT column tiles: the smallest form that takes all rows in one pass, 64 rows a pass beyond. Blocks of a cluster share K: more of them for
-// longer rows, so that the slice of x fits, and for matrices of so few tiles that the warps of fewer blocks would stand idle.
+// Clusters of cs blocks that are resident at once, with one block a multiprocessor and with two: a property of the device, asked once.
+static int g_clusters[32][2][4];
+
+// The rows of x decide NT, up to 32 a pass. Blocks of a cluster (cs) and warps of a block (kw) share K. Of all splits whose slice of x fits, the one
+// with the least work on a warp's way: batches of tiles, each (in halves of a step) its steps and about three steps of a
+// batch's end, which grows with the slices whose sums meet there.
 template <bool F16, int NT>
 static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 32) return -2;
   const int groups = p.k / 128, mt = (p.n + 15) / 16, passes = (p.rows + 8 * NT - 1) / (8 * NT);
-  int cs = 1;
-  while (cs < 8 && 2 * cs <= groups && (Shape<NT>::bytes(128 * ((groups + cs - 1) / cs)) > SMEM_MAX || (long long)mt * passes * cs < (long long)CW * dev.sms)) cs *= 2;
+  int cs = 8, kw = 1, clusters = 1;
+  long long least = -1;
+  for (int lg = 0; lg < 4 && 1 << lg <= groups; ++lg) {
+    const int slice = (groups + (1 << lg) - 1) >> lg;
+    const size_t bytes = Shape<NT>::bytes(128 * slice);
+    if (bytes > SMEM_MAX) continue;
+    const int avail = g_clusters[d][bytes <= SMEM_TWO][lg] / passes;
+    for (int w = 1; w <= 4 && w <= slice; w *= 2) {
+      const int need = (int)(((long long)mt * w + CW - 1) / CW), have = avail < 1 ? 1 : avail < need ? avail : need;
+      const int waves = avail < 1 ? (passes + g_clusters[d][bytes <= SMEM_TWO][lg] - 1) / g_clusters[d][bytes <= SMEM_TWO][lg] : 1;
+      const long long cost = (long long)waves * ((need + have - 1) / have) * (2 * ((slice + w - 1) / w) + 6 + w * (1 << lg) / 2);
+      if (least < 0 || cost < least) least = cost, cs = 1 << lg, kw = w, clusters = have;
+    }
+  }
   const size_t smem = Shape<NT>::bytes(128 * ((groups + cs - 1) / cs));
-  int clusters = dev.sms / cs / passes;
-  if (clusters < 1) clusters = 1;
-  if (clusters > (mt + CW - 1) / CW) clusters = (mt + CW - 1) / CW;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * cs, passes);
   cfg.blockDim = dim3(THREADS);
@@ -294,17 +474,19 @@ static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = dev.pdl ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, k_proj<F16, NT>, p);
+  cudaLaunchKernelEx(&cfg, k_proj<F16, NT>, p, kw, 2 * 128 * ((groups + cs - 1) / cs) + 16);
   return 0;
 }
 
 template <bool F16>
 static int launch_any(const Args& p, const DrbDevice& dev, cudaStream_t st) {
-  if (p.rank > 0) drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
+  if (p.rank > 0) {
+    if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
+    else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
+  }
   if (p.rows <= 8) return launch<F16, 1>(p, dev, st);
   if (p.rows <= 16) return launch<F16, 2>(p, dev, st);
-  if (p.rows <= 32) return launch<F16, 4>(p, dev, st);
-  return launch<F16, 8>(p, dev, st);
+  return launch<F16, 4>(p, dev, st);
 }
 
 template <bool F16, int NT>
@@ -318,12 +500,26 @@ static cudaError_t configure_type() {
   if ((e = configure<F16, 1>()) != cudaSuccess) return e;
   if ((e = configure<F16, 2>()) != cudaSuccess) return e;
   if ((e = configure<F16, 4>()) != cudaSuccess) return e;
-  if ((e = configure<F16, 8>()) != cudaSuccess) return e;
+  if ((e = drb_carveout(k_shrink_rows<F16>)) != cudaSuccess) return e;
   return drb_carveout(k_shrink<F16>);
 }
 static cudaError_t configure_all() {
-  const cudaError_t e = configure_type<false>();
-  return e != cudaSuccess ? e : configure_type<true>();
+  cudaError_t e = configure_type<false>();
+  if (e != cudaSuccess || (e = configure_type<true>()) != cudaSuccess) return e;
+  int d = 0;
+  if ((e = cudaGetDevice(&d)) != cudaSuccess) return e;
+  if (d < 0 || d >= 32) return cudaErrorInvalidDevice;
+  for (int two = 0; two < 2; ++two)
+    for (int lg = 0; lg < 4; ++lg) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1 << lg), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = two ? SMEM_TWO : SMEM_MAX;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1 << lg, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr, cfg.numAttrs = 1;
+      if ((e = cudaOccupancyMaxActiveClusters(&g_clusters[d][two][lg], k_proj<true, 4>, &cfg)) != cudaSuccess) return e;
+    }
+  return cudaSuccess;
 }
 
 }  // namespace pl
