@@ -172,11 +172,6 @@ __global__ void __launch_bounds__(256) k_shrink_rows(Args p) {
 }
 
 // ---- y = W x + res + B v -----------------------------------------------------------------------------------------------
-DRB_DEV unsigned cluster_size() {
-  unsigned v;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(v));
-  return v;
-}
 DRB_DEV unsigned cluster_rank() {
   unsigned v;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(v));
@@ -196,7 +191,7 @@ DRB_DEV float4 ld_peer(uint32_t addr, unsigned rank) {
 template <int NT>
 struct Shape {
   static constexpr size_t SUMS = (size_t)CW * 8 * NT * PP * 4, RING = (size_t)CW * DEPTH * SUB;
-  static constexpr size_t VS = (size_t)8 * NT * (MAX_RANK + 4) * 4;  // v of the pass, where the tensor cores take it
+  static constexpr size_t VS = (size_t)8 * NT * (MAX_RANK + 4) * 4;  // v of the pass
   static constexpr size_t bytes(int slice) { return 256 + (size_t)8 * NT * (2 * slice + 16) + SUMS + RING + VS; }
 };
 static_assert(Shape<4>::bytes(MAX_K / 8) <= SMEM_MAX, "eight blocks hold the longest row");
@@ -212,27 +207,34 @@ DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
   }
 }
 
-// blockIdx.y: the pass of 8 NT rows of x. Cluster c of the pass owns weight tiles [mt c / C, mt (c + 1) / C), kw warps of a block share a tile.
+// How a launch shares out its tiles and K: `each` tiles a cluster and one more for the first `more`; clusters of 1 << lcs blocks, 1 << lkw warps a
+// tile. All divisions are made on the host (a few dozen runtime divisions a thread took 3 us of 15).
+struct Split {
+  int each, more, lcs, lkw, pitch;
+};
+
+// blockIdx.y: the pass of 8 NT rows of x.
 template <bool F16, int NT>
-__global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) {
+__global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   extern __shared__ __align__(128) unsigned char dyn[];
   int* who = reinterpret_cast<int*>(dyn);  // [8 NT] adapters of the pass's rows, then the different ones among them and their number
   unsigned char* xs = dyn + 256;
-  float* sums = reinterpret_cast<float*>(xs + (size_t)8 * NT * pitch);
+  float* sums = reinterpret_cast<float*>(xs + (size_t)8 * NT * sp.pitch);
   float* vs = sums + Shape<NT>::SUMS / 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(vs) + Shape<NT>::VS + warp * DEPTH * SUB;
-  const int cs = (int)cluster_size(), cr = (int)cluster_rank(), C = (int)gridDim.x / cs, c = (int)blockIdx.x / cs;
-  const int tw = CW / kw, wt = warp / kw, wk = warp % kw;                                   // tiles of a batch; this warp's tile and share of K
-  const int groups = p.k / 128, b0 = groups * cr / cs, bn = groups * (cr + 1) / cs - b0;    // this block's inputs, in 128s
-  const int g0 = bn * wk / kw, ng = bn * (wk + 1) / kw - g0;                                // this warp's, of the block's
-  const int mt = (p.n + 15) / 16, t0 = (int)((long long)mt * c / C), t1 = (int)((long long)mt * (c + 1) / C);
+  const int lcs = sp.lcs, lkw = sp.lkw, cs = 1 << lcs, kw = 1 << lkw, pitch = sp.pitch;
+  const int cr = (int)cluster_rank(), c = (int)blockIdx.x >> lcs;
+  const int tw = CW >> lkw, wt = warp >> lkw, wk = warp & (kw - 1);                               // tiles of a batch; this warp's tile and share of K
+  const int groups = p.k >> 7, b0 = groups * cr >> lcs, bn = (groups * (cr + 1) >> lcs) - b0;     // this block's inputs, in 128s
+  const int g0 = bn * wk >> lkw, ng = (bn * (wk + 1) >> lkw) - g0;                                // this warp's, of the block's
+  const int t0 = sp.each * c + min(sp.more, c), t1 = t0 + sp.each + (c < sp.more ? 1 : 0);
   const int row0 = (int)blockIdx.y * 8 * NT, cols = min(8 * NT, p.rows - row0);
 
   pdl_launch_dependents();
 
   // The weights' stream: tiles t0 + wt, t0 + wt + tw, ..., ng steps each. Rows behind the last one are read as the last one.
-  const int mine = t1 - t0 > wt ? (t1 - t0 - wt + tw - 1) / tw : 0;
+  const int mine = t1 - t0 > wt ? (t1 - t0 - wt + tw - 1) >> (3 - lkw) : 0;
   int nslot = 0, slot = 0, ltile = t0 + wt, lg = 0, left = mine * ng;
   const uint32_t put = (lane >> 3) * 128 + 16 * ((lane & 7) ^ (((lane >> 3) & 1) << 2));
   const int8_t* src = p.w;  // this lane's piece of the next step in row 16 ltile, and its four rows from there
@@ -241,6 +243,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
     src = p.w + (size_t)16 * ltile * p.k + (b0 + g0) * 128 + 16 * (lane & 7);
 #pragma unroll
     for (int i = 0; i < 4; ++i) over[i] = min((lane >> 3) + 4 * i, p.n - 1 - 16 * ltile) * p.k;
+    // the tile's scales, which are read a step ahead of use, come to L2 with its first weights
+    if (lane < 16) prefetch_line_l2(p.s + (size_t)min(16 * ltile + lane, p.n - 1) * groups + b0 + g0);
   };
   if (left > 0) aim();
   auto issue = [&]() {
@@ -260,19 +264,18 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
   };
 #pragma unroll 1
   for (int i = 0; i < DEPTH; ++i) issue();
-  auto scales = [&](int tile, int grp, float& s0, float& s1) {
-    s0 = __half2float(__ldg(p.s + (size_t)min(16 * tile + g, p.n - 1) * groups + b0 + g0 + grp));
-    s1 = __half2float(__ldg(p.s + (size_t)min(16 * tile + g + 8, p.n - 1) * groups + b0 + g0 + grp));
+  __half s0 = __half(), s1 = __half();  // the next step's; converted when they are used, so that nothing waits for them before
+  auto scales = [&](int tile, int grp) {
+    s0 = __ldg(p.s + (size_t)min(16 * tile + g, p.n - 1) * groups + b0 + g0 + grp);
+    s1 = __ldg(p.s + (size_t)min(16 * tile + g + 8, p.n - 1) * groups + b0 + g0 + grp);
   };
-  float s0 = 0.f, s1 = 0.f;
-  if (mine * ng > 0) scales(t0 + wt, 0, s0, s1);
+  if (mine * ng > 0) scales(t0 + wt, 0);
 
   if (p.rank == 0) pdl_wait();  // with adapters x and the rest are older than k_shrink, and only v is awaited, below
   {
-    const int pieces = bn * 16;  // of 16 bytes a row
-    for (int i = threadIdx.x; i < 8 * NT * pieces; i += THREADS) {
-      const int r = i / pieces, q = i - r * pieces;
-      few::cp16(smem_u32(xs + r * pitch + 16 * q), static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(r, cols - 1)) * p.k + b0 * 128 + 8 * q);
+    for (int r = warp; r < 8 * NT; r += CW) {  // a warp a row, 16 bytes a lane
+      const uint16_t* src = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(r, cols - 1)) * p.k + b0 * 128;
+      for (int q = lane; q < 16 * bn; q += 32) few::cp16(smem_u32(xs) + r * pitch + 16 * q, src + 8 * q);
     }
     few::cp_commit();
     if (p.rank > 0 && threadIdx.x < 8 * NT) {
@@ -291,8 +294,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
     if (warp == 0 && (firsts >> lane) & 1u) who[32 + __popc(firsts & ((1u << lane) - 1u))] = a;
   }
   const bool tensor = ndiff > 0 && ndiff <= TENSOR_ADAPTERS && p.rows > TILE_ROWS;
+  // Without them: a warp takes the sixteen weight rows of a tile for a row of x, two lanes a weight row; the pairs of a batch are dealt out
+  // over the cluster and its warps. The rows of B for the first batch come to L2 meanwhile.
+  const int lr = lane >> 1, half = lane & 1;
+  auto pair_row = [&](int tile, int r) { return p.b + ((size_t)who[r] * p.n + min(16 * tile + lr, p.n - 1)) * p.rank; };
+  if (ndiff > 0 && !tensor)
+    for (int i = cr * CW + warp; i < min(tw, t1 - t0) * 8 * NT; i += cs * CW)
+      if (who[i % (8 * NT)] >= 0 && 64 * half < p.rank) prefetch_line_l2(pair_row(t0 + i / (8 * NT), i % (8 * NT)) + 32 * half);
 
-  const int batches = (t1 - t0 + tw - 1) / tw;
+  const int batches = (t1 - t0 + tw - 1) >> (3 - lkw);
   const uint32_t xb = smem_u32(xs) + g * pitch + 32 * t + 256 * g0;
   for (int bt = 0; bt < batches; ++bt) {
     const int tile = t0 + bt * tw + wt;
@@ -302,9 +312,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
     if (tile < t1) {
 #pragma unroll 1
       for (int q = 0; q < ng; ++q) {
-        const float f0 = s0, f1 = s1;
-        if (q + 1 < ng) scales(tile, q + 1, s0, s1);
-        else if (tile + tw < t1) scales(tile + tw, 0, s0, s1);
+        const __half h0 = s0, h1 = s1;
+        if (q + 1 < ng) scales(tile, q + 1);
+        else if (tile + tw < t1) scales(tile + tw, 0);
         few::cp_wait<DEPTH - 1>();
         __syncwarp();
         const uint32_t r0 = ring + slot * SUB + g * 128 + 64 * (g & 1) + 16 * t;
@@ -333,6 +343,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
         __syncwarp();
         issue();
         if (++slot == DEPTH) slot = 0;
+        const float f0 = __half2float(h0), f1 = __half2float(h1);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           acc[i][0] = fmaf(f0, d[i][0], acc[i][0]), acc[i][1] = fmaf(f0, d[i][1], acc[i][1]);
@@ -342,9 +353,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
     }
     if (p.rank > 0 && bt == 0) {
       pdl_wait();  // v
-      if (tensor) {
-        for (int i = threadIdx.x; i < 8 * NT * (p.rank / 4); i += THREADS) {
-          const int r = i / (p.rank / 4), q = i % (p.rank / 4);
+      if (ndiff > 0) {
+        for (int i = threadIdx.x; i < 8 * NT * (MAX_RANK / 4); i += THREADS) {
+          const int r = i / (MAX_RANK / 4), q = i % (MAX_RANK / 4);
+          if (4 * q >= p.rank) continue;
           *reinterpret_cast<float4*>(vs + r * (MAX_RANK + 4) + 4 * q) =
               r < cols && who[r] >= 0 ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -353,10 +365,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
     }
     if (tensor && tile < t1) {
       // B v as more inputs: sixteen ranks of an adapter at a time, dealt out over the K slices; rows of other adapters count as zeros
-      const int chunks = (p.rank + 15) / 16;
 #pragma unroll 1
-      for (int i0 = cr * kw + wk; i0 < ndiff * chunks; i0 += cs * kw) {
-        const int ad = who[32 + i0 / chunks], k0 = i0 % chunks * 16 + 4 * t;
+      for (int i0 = cr * kw + wk; i0 < ndiff * (MAX_RANK / 16); i0 += cs * kw) {
+        if (i0 % (MAX_RANK / 16) * 16 >= p.rank) continue;
+        const int ad = who[32 + i0 / (MAX_RANK / 16)], k0 = i0 % (MAX_RANK / 16) * 16 + 4 * t;
         uint2 u = make_uint2(0u, 0u), v = u;
         const bool in = k0 < p.rank;
         if (in) {
@@ -382,41 +394,57 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
       st[(8 * i + 2 * t) * PP + g] = acc[i][0], st[(8 * i + 2 * t + 1) * PP + g] = acc[i][1];
       st[(8 * i + 2 * t) * PP + g + 8] = acc[i][2], st[(8 * i + 2 * t + 1) * PP + g + 8] = acc[i][3];
     }
+    const int nt = min(tw, t1 - t0 - bt * tw);
+    if (ndiff > 0 && !tensor) {
+      __syncthreads();
+      constexpr int PAIRS = 8;  // on the way at once
+      for (int i0 = cr * CW + warp; i0 < nt * 8 * NT; i0 += PAIRS * cs * CW) {
+        float a[PAIRS];
+        const uint4* bp[PAIRS];
+        int r[PAIRS];
+#pragma unroll
+        for (int e = 0; e < PAIRS; ++e) {
+          const int i = i0 + e * cs * CW;
+          r[e] = i % (8 * NT), a[e] = 0.f;
+          bp[e] = who[r[e]] < 0 || i >= nt * 8 * NT ? nullptr : reinterpret_cast<const uint4*>(pair_row(t0 + bt * tw + i / (8 * NT), r[e])) + half;
+        }
+        for (int q = half; q < p.rank / 8; q += 2) {
+          uint4 bw[PAIRS];
+#pragma unroll
+          for (int e = 0; e < PAIRS; ++e) bw[e] = bp[e] ? __ldcg(bp[e] + (q - half)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int e = 0; e < PAIRS; ++e) {
+            const float4* vp = reinterpret_cast<const float4*>(vs + r[e] * (MAX_RANK + 4) + 8 * q);
+            const float4 v0 = vp[0], v1 = vp[1];
+            a[e] = fmaf(widen16(bw[e].x & 0xffffu, false), v0.x, a[e]), a[e] = fmaf(widen16(bw[e].x >> 16, false), v0.y, a[e]);
+            a[e] = fmaf(widen16(bw[e].y & 0xffffu, false), v0.z, a[e]), a[e] = fmaf(widen16(bw[e].y >> 16, false), v0.w, a[e]);
+            a[e] = fmaf(widen16(bw[e].z & 0xffffu, false), v1.x, a[e]), a[e] = fmaf(widen16(bw[e].z >> 16, false), v1.y, a[e]);
+            a[e] = fmaf(widen16(bw[e].w & 0xffffu, false), v1.z, a[e]), a[e] = fmaf(widen16(bw[e].w >> 16, false), v1.w, a[e]);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < PAIRS; ++e) {
+          const float both = a[e] + __shfl_xor_sync(0xffffffffu, a[e], 1);
+          if (half == 0 && bp[e]) sums[((i0 + e * cs * CW) / (8 * NT) * kw * 8 * NT + r[e]) * PP + lr] += both;
+        }
+      }
+    }
     __syncwarp();
     cluster_arrive();
     cluster_wait();
     // Block cr of the cluster finishes its share of the batch, four weight rows of a column (a row of x) at a time
-    const int nt = min(tw, t1 - t0 - bt * tw), outs = nt * 4 * cols;
-    for (int i = outs * cr / cs + (int)threadIdx.x; i < outs * (cr + 1) / cs; i += THREADS) {
-      const int j = 4 * (i & 3), m = (i >> 2) % nt, r = (i >> 2) / nt, o = 16 * (t0 + bt * tw + m) + j, row = row0 + r;
-      if (o >= p.n) continue;
-      const int ad = p.rank > 0 && !tensor ? who[r] : -1;
-      float4 f[8];
+    for (int i = cr * THREADS + (int)threadIdx.x; i < tw * 4 * cols; i += cs * THREADS) {
+      const int j = 4 * (i & 3), m = (i >> 2) & (tw - 1), r = i >> (5 - lkw), o = 16 * (t0 + bt * tw + m) + j, row = row0 + r;
+      if (m >= nt || o >= p.n) continue;
       const uint32_t at = smem_u32(sums + (m * kw * 8 * NT + r) * PP + j);
       float v[4] = {0.f, 0.f, 0.f, 0.f};
       for (int k = 0; k < kw; ++k) {
+        float4 f[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) f[q] = q < cs ? ld_peer(at + k * 8 * NT * PP * 4, (unsigned)q) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[0] += f[q].x, v[1] += f[q].y, v[2] += f[q].z, v[3] += f[q].w;
-      }
-      if (ad >= 0) {
-        const float4* vp = reinterpret_cast<const float4*>(p.v + (size_t)row * p.rank);
-        const uint4* bp = reinterpret_cast<const uint4*>(p.b + ((size_t)ad * p.n + o) * p.rank);
-        const int r8 = p.rank / 8;
-        for (int q = 0; q < r8; ++q) {
-          const float4 v0 = __ldcg(vp + 2 * q), v1 = __ldcg(vp + 2 * q + 1);
-          uint4 bw[4];
-#pragma unroll
-          for (int l = 0; l < 4; ++l) bw[l] = __ldcg(bp + min(l, p.n - 1 - o) * r8 + q);
-#pragma unroll
-          for (int l = 0; l < 4; ++l) {
-            v[l] = fmaf(widen16(bw[l].x & 0xffffu, false), v0.x, v[l]), v[l] = fmaf(widen16(bw[l].x >> 16, false), v0.y, v[l]);
-            v[l] = fmaf(widen16(bw[l].y & 0xffffu, false), v0.z, v[l]), v[l] = fmaf(widen16(bw[l].y >> 16, false), v0.w, v[l]);
-            v[l] = fmaf(widen16(bw[l].z & 0xffffu, false), v1.x, v[l]), v[l] = fmaf(widen16(bw[l].z >> 16, false), v1.y, v[l]);
-            v[l] = fmaf(widen16(bw[l].w & 0xffffu, false), v1.z, v[l]), v[l] = fmaf(widen16(bw[l].w >> 16, false), v1.w, v[l]);
-          }
-        }
       }
       const size_t yo = (size_t)row * p.n + o;
       if (p.n % 4 == 0 && (((uintptr_t)p.y | (uintptr_t)p.res) & 15) == 0) {
@@ -440,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, int kw, int pitch) 
 static int g_clusters[32][2][4];
 
 // The rows of x decide NT, up to 32 a pass. Blocks of a cluster (cs) and warps of a block (kw) share K. Of all splits whose slice of x fits, the one
-// with the least work on a warp's way: batches of tiles, each (in halves of a step) its steps and about three steps of a
+// with the least work on a warp's way (of equals the widest cluster, whose blocks read least of x): batches of tiles, each (in halves of a step) its steps and about three steps of a
 // batch's end, which grows with the slices whose sums meet there.
 template <bool F16, int NT>
 static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
@@ -458,7 +486,7 @@ static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
       const int need = (int)(((long long)mt * w + CW - 1) / CW), have = avail < 1 ? 1 : avail < need ? avail : need;
       const int waves = avail < 1 ? (passes + g_clusters[d][bytes <= SMEM_TWO][lg] - 1) / g_clusters[d][bytes <= SMEM_TWO][lg] : 1;
       const long long cost = (long long)waves * ((need + have - 1) / have) * (2 * ((slice + w - 1) / w) + 6 + w * (1 << lg) / 2);
-      if (least < 0 || cost < least) least = cost, cs = 1 << lg, kw = w, clusters = have;
+      if (least < 0 || cost <= least) least = cost, cs = 1 << lg, kw = w, clusters = have;
     }
   }
   const size_t smem = Shape<NT>::bytes(128 * ((groups + cs - 1) / cs));
@@ -474,7 +502,9 @@ static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = dev.pdl ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, k_proj<F16, NT>, p, kw, 2 * 128 * ((groups + cs - 1) / cs) + 16);
+  const auto lg2 = [](int v) { return v == 1 ? 0 : v == 2 ? 1 : v == 4 ? 2 : 3; };
+  const Split sp = {mt / clusters, mt % clusters, lg2(cs), lg2(kw), 2 * 128 * ((groups + cs - 1) / cs) + 16};
+  cudaLaunchKernelEx(&cfg, k_proj<F16, NT>, p, sp);
   return 0;
 }
 
