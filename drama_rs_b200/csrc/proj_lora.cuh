@@ -272,35 +272,48 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   if (mine * ng > 0) scales(t0 + wt, 0);
 
   if (p.rank == 0) pdl_wait();  // with adapters x and the rest are older than k_shrink, and only v is awaited, below
+  // x by plain loads, so that nothing here waits for the weights: a warp takes NT rows, 16 bytes a lane, two pieces of each at once
+  const int ad = p.rank > 0 && lane < cols ? adapter(p, row0 + lane) : -1;  // lane r: of row r
   {
-    for (int r = warp; r < 8 * NT; r += CW) {  // a warp a row, 16 bytes a lane
-      const uint16_t* src = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(r, cols - 1)) * p.k + b0 * 128;
-      for (int q = lane; q < 16 * bn; q += 32) few::cp16(smem_u32(xs) + r * pitch + 16 * q, src + 8 * q);
+    const uint4* src[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) src[i] = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(warp + CW * i, cols - 1)) * p.k + b0 * 128);
+    for (int q = lane; q < 16 * bn; q += 64) {
+      uint4 v[2][NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        v[0][i] = __ldcg(src[i] + q);
+        if (q + 32 < 16 * bn) v[1][i] = __ldcg(src[i] + q + 32);
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        uint4* dst = reinterpret_cast<uint4*>(xs + (warp + CW * i) * pitch);
+        dst[q] = v[0][i];
+        if (q + 32 < 16 * bn) dst[q + 32] = v[1][i];
+      }
     }
-    few::cp_commit();
-    if (p.rank > 0 && threadIdx.x < 8 * NT) {
-      const int a = (int)threadIdx.x < cols ? adapter(p, row0 + threadIdx.x) : -1;
-      who[threadIdx.x] = a;
-    }
-    few::cp_wait<0>();
-    __syncthreads();
   }
   int ndiff = 0;
   if (p.rank > 0) {  // the different adapters, in every warp for itself
-    const int a = lane < 8 * NT ? who[lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, a);
-    const unsigned firsts = __ballot_sync(0xffffffffu, a >= 0 && __ffs(same) - 1 == lane);
+    const unsigned same = __match_any_sync(0xffffffffu, ad);
+    const unsigned firsts = __ballot_sync(0xffffffffu, ad >= 0 && __ffs(same) - 1 == lane);
     ndiff = __popc(firsts);
-    if (warp == 0 && (firsts >> lane) & 1u) who[32 + __popc(firsts & ((1u << lane) - 1u))] = a;
+    if (warp == 0) {
+      who[lane] = ad;
+      if ((firsts >> lane) & 1u) who[32 + __popc(firsts & ((1u << lane) - 1u))] = ad;
+    }
   }
   const bool tensor = ndiff > 0 && ndiff <= TENSOR_ADAPTERS && p.rows > TILE_ROWS;
   // Without them: a warp takes the sixteen weight rows of a tile for a row of x, two lanes a weight row; the pairs of a batch are dealt out
   // over the cluster and its warps. The rows of B for the first batch come to L2 meanwhile.
   const int lr = lane >> 1, half = lane & 1;
-  auto pair_row = [&](int tile, int r) { return p.b + ((size_t)who[r] * p.n + min(16 * tile + lr, p.n - 1)) * p.rank; };
+  auto pair_row = [&](int tile, int a) { return p.b + ((size_t)a * p.n + min(16 * tile + lr, p.n - 1)) * p.rank; };
   if (ndiff > 0 && !tensor)
-    for (int i = cr * CW + warp; i < min(tw, t1 - t0) * 8 * NT; i += cs * CW)
-      if (who[i % (8 * NT)] >= 0 && 64 * half < p.rank) prefetch_line_l2(pair_row(t0 + i / (8 * NT), i % (8 * NT)) + 32 * half);
+    for (int i = cr * CW + warp; i < min(tw, t1 - t0) * 8 * NT; i += cs * CW) {
+      const int a = __shfl_sync(0xffffffffu, ad, i % (8 * NT));
+      if (a >= 0 && 64 * half < p.rank) prefetch_line_l2(pair_row(t0 + i / (8 * NT), a) + 32 * half);
+    }
+  __syncthreads();
 
   const int batches = (t1 - t0 + tw - 1) >> (3 - lkw);
   const uint32_t xb = smem_u32(xs) + g * pitch + 32 * t + 256 * g0;
@@ -406,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
         for (int e = 0; e < PAIRS; ++e) {
           const int i = i0 + e * cs * CW;
           r[e] = i % (8 * NT), a[e] = 0.f;
-          bp[e] = who[r[e]] < 0 || i >= nt * 8 * NT ? nullptr : reinterpret_cast<const uint4*>(pair_row(t0 + bt * tw + i / (8 * NT), r[e])) + half;
+          bp[e] = who[r[e]] < 0 || i >= nt * 8 * NT ? nullptr : reinterpret_cast<const uint4*>(pair_row(t0 + bt * tw + i / (8 * NT), who[r[e]])) + half;
         }
         for (int q = half; q < p.rank / 8; q += 2) {
           uint4 bw[PAIRS];
@@ -516,6 +529,7 @@ static int launch_any(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   }
   if (p.rows <= 8) return launch<F16, 1>(p, dev, st);
   if (p.rows <= 16) return launch<F16, 2>(p, dev, st);
+  if (p.rows <= 24) return launch<F16, 3>(p, dev, st);
   return launch<F16, 4>(p, dev, st);
 }
 
@@ -529,6 +543,7 @@ static cudaError_t configure_type() {
   cudaError_t e;
   if ((e = configure<F16, 1>()) != cudaSuccess) return e;
   if ((e = configure<F16, 2>()) != cudaSuccess) return e;
+  if ((e = configure<F16, 3>()) != cudaSuccess) return e;
   if ((e = configure<F16, 4>()) != cudaSuccess) return e;
   if ((e = drb_carveout(k_shrink_rows<F16>)) != cudaSuccess) return e;
   return drb_carveout(k_shrink<F16>);
