@@ -522,15 +522,17 @@ static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
 }
 
 template <bool F16>
-static int launch_any(const Args& p, const DrbDevice& dev, cudaStream_t st) {
-  if (p.rank > 0) {
-    if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
-    else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
-  }
+static int launch_few(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   if (p.rows <= 8) return launch<F16, 1>(p, dev, st);
   if (p.rows <= 16) return launch<F16, 2>(p, dev, st);
   if (p.rows <= 24) return launch<F16, 3>(p, dev, st);
   return launch<F16, 4>(p, dev, st);
+}
+
+template <bool F16>
+static void launch_shrink(const Args& p, const DrbDevice& dev, cudaStream_t st) {
+  if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
+  else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
 }
 
 template <bool F16, int NT>
@@ -568,20 +570,3 @@ static cudaError_t configure_all() {
 }
 
 }  // namespace pl
-
-extern "C" int drb_proj_q8_lora(const int8_t* w, const __half* s, const void* x, int x_type, const __nv_bfloat16* a, const __nv_bfloat16* b,
-                                const float* scale, const int* adapter_of, int adapters, int rank, const float* res, float* y, float* v, int rows, int n,
-                                int k, cudaStream_t st) {
-  if ((x_type != 1 && x_type != 2) || rows < 0 || n < 1 || k < 128 || k > pl::MAX_K || k % 128 || rank < 0 || rank > pl::MAX_RANK || rank % 8 || adapters < 0)
-    return -1;
-  if (!w || !s || !x || !y || (rank > 0 && (!a || !b || !scale || !adapter_of || !v))) return -1;
-  const auto off = [](const void* p, unsigned m) { return ((uintptr_t)p & (m - 1)) != 0; };
-  if (off(w, 16) || off(s, 2) || off(x, 16) || off(y, 4) || off(res, 4)) return -3;
-  if (rank > 0 && (off(a, 16) || off(b, 16) || off(v, 16) || off(scale, 4) || off(adapter_of, 4))) return -3;
-  const DrbDevice& dev = drb_device(st);
-  if (!dev.ready) return -2;
-  if (rows == 0) return 0;
-  if (rows > 65535 * 64) return -1;
-  const pl::Args p = {w, s, x, a, b, scale, res, adapter_of, y, v, adapters, adapters > 0 ? rank : 0, rows, n, k};
-  return x_type == 2 ? pl::launch_any<true>(p, dev, st) : pl::launch_any<false>(p, dev, st);
-}

@@ -32,6 +32,7 @@ namespace pft { static cudaError_t configure_all(); }
 namespace bn { static cudaError_t configure_all(); }
 namespace few { static cudaError_t configure_all(); }
 namespace pl { static cudaError_t configure_all(); }
+namespace pr { static cudaError_t configure_all(); }
 
 namespace rt {
 
@@ -60,6 +61,7 @@ static cudaError_t setup(int d) {
   if ((e = bn::configure_all()) != cudaSuccess) return e;
   if ((e = few::configure_all()) != cudaSuccess) return e;
   if ((e = pl::configure_all()) != cudaSuccess) return e;
+  if ((e = pr::configure_all()) != cudaSuccess) return e;
   dv.ready = true;
   g_dev[d] = dv;
   g_ready[d].store(true, std::memory_order_release);
