@@ -3,8 +3,8 @@
 //   y_r = W x_r (+ res_r) + scale_a B_a (A_a x_r),  a = adapter_of[r]
 //
 // Two launches (one without adapters). v_r = scale_a A_a x_r: k_shrink, a warp a dot product, or k_shrink_rows, sixteen rows a block on the
-// tensor cores. Then k_proj: the weights' stream, with the adapters' second half on its sums. Bound by the bytes of W and of the
-// adapters hit for few rows; from some 64 rows on by mma.sync.
+// tensor cores. Then the weights' stream, with the adapters' second half on its sums: k_proj up to 64 rows, k_proj_rows (tcgen05) beyond.
+// Bound by the bytes of W and of the adapters hit for few rows, by the conversion of the codes for many.
 //
 // k_proj: 16-bit x meets the int8 codes, which both 16-bit types hold exactly, on mma.sync m16n8k16; a sum over the 128 inputs of a weight
 // scale is fp32, scaled in fp32, so no weight is rounded. The 16 weight rows of a tile are M, the rows of x are N (8 to 32 a pass). A
@@ -26,8 +26,7 @@ constexpr int SUB = 2048;                  // a step of a warp: 16 weight rows x
 constexpr int DEPTH = 3;
 constexpr int PP = 20;                     // floats between the columns of a tile of sums: writes of a warp meet no bank twice
 constexpr size_t SMEM_MAX = 232448, SMEM_TWO = 112 * 1024;  // up to the second, two blocks share a multiprocessor
-constexpr int TILE_ROWS = 64;              // more rows than these: k_shrink_rows
-constexpr int TENSOR_ADAPTERS = 4;         // adapters in a pass up to which their second half runs on the tensor cores
+constexpr int TILE_ROWS = 64;              // up to so many rows: k_shrink and k_proj, beyond: k_shrink_rows and k_proj_rows
 
 struct Args {
   const int8_t* w;
@@ -122,46 +121,52 @@ DRB_DEV void split_f16(uint32_t h, uint32_t& hi, uint32_t& lo) {
 // Rows are M, ranks are N; both operands straight from L2. fp16 rows meet the bf16 adapters as two bf16 terms.
 template <bool F16>
 __global__ void __launch_bounds__(256) k_shrink_rows(Args p) {
-  __shared__ int who[16];
   __shared__ float part[8][16][8];
   const int row0 = (int)blockIdx.x * 16, j0 = (int)blockIdx.y * 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rows = min(16, p.rows - row0);
   pdl_wait();
   pdl_launch_dependents();
-  if (threadIdx.x < 16) who[threadIdx.x] = (int)threadIdx.x < rows ? adapter(p, row0 + threadIdx.x) : -1;
-  __syncthreads();
+  const int who = lane < rows ? adapter(p, row0 + lane) : -1;  // lane r: of row r
+  const unsigned same = __match_any_sync(0xffffffffu, who);
+  unsigned firsts = __ballot_sync(0xffffffffu, who >= 0 && __ffs(same) - 1 == lane);
   const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(g, rows - 1)) * p.k + 8 * t;
   const uint16_t* x1 = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(g + 8, rows - 1)) * p.k + 8 * t;
   const int steps = p.k / 32, c0 = steps * warp / 8, c1 = steps * (warp + 1) / 8;
-  for (int r = 0; r < rows; ++r) {
-    const int ad = who[r];
-    bool seen = ad < 0;
-    for (int q = 0; q < r; ++q) seen |= who[q] == ad;
-    if (seen) continue;  // the same in every thread
+  for (; firsts; firsts &= firsts - 1u) {  // the different adapters
+    const int r = __ffs(firsts) - 1, ad = __shfl_sync(0xffffffffu, who, r);
+    const unsigned mine = __shfl_sync(0xffffffffu, same, r);
     const uint16_t* ap = reinterpret_cast<const uint16_t*>(p.a) + ((size_t)ad * p.rank + j0 + g) * p.k + 8 * t;
     float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int c = c0; c < c1; ++c) {
-      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(x0 + 32 * c)), v = __ldcg(reinterpret_cast<const uint4*>(x1 + 32 * c));
-      const uint4 b = __ldcg(reinterpret_cast<const uint4*>(ap + 32 * c));
-      if constexpr (F16) {
-        uint32_t uh[4], ul[4], vh[4], vl[4];
-        split_f16(u.x, uh[0], ul[0]), split_f16(u.y, uh[1], ul[1]), split_f16(u.z, uh[2], ul[2]), split_f16(u.w, uh[3], ul[3]);
-        split_f16(v.x, vh[0], vl[0]), split_f16(v.y, vh[1], vl[1]), split_f16(v.z, vh[2], vl[2]), split_f16(v.w, vh[3], vl[3]);
-        mma16<false>(d, uh[0], vh[0], uh[1], vh[1], b.x, b.y);
-        mma16<false>(e, uh[2], vh[2], uh[3], vh[3], b.z, b.w);
-        mma16<false>(d, ul[0], vl[0], ul[1], vl[1], b.x, b.y);
-        mma16<false>(e, ul[2], vl[2], ul[3], vl[3], b.z, b.w);
-      } else {
-        mma16<false>(d, u.x, v.x, u.y, v.y, b.x, b.y);
-        mma16<false>(e, u.z, v.z, u.w, v.w, b.z, b.w);
+    constexpr int FLY = F16 ? 4 : 8;  // pieces on the way at once
+    for (int c = c0; c < c1; c += FLY) {
+      uint4 u[FLY], v[FLY], b[FLY];
+#pragma unroll
+      for (int q = 0; q < FLY; ++q) {
+        const int at = 32 * min(c + q, c1 - 1);
+        u[q] = __ldcg(reinterpret_cast<const uint4*>(x0 + at)), v[q] = __ldcg(reinterpret_cast<const uint4*>(x1 + at));
+        b[q] = c + q < c1 ? __ldcg(reinterpret_cast<const uint4*>(ap + at)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int q = 0; q < FLY; ++q) {
+        if constexpr (F16) {
+          uint32_t uh[4], ul[4], vh[4], vl[4];
+          split_f16(u[q].x, uh[0], ul[0]), split_f16(u[q].y, uh[1], ul[1]), split_f16(u[q].z, uh[2], ul[2]), split_f16(u[q].w, uh[3], ul[3]);
+          split_f16(v[q].x, vh[0], vl[0]), split_f16(v[q].y, vh[1], vl[1]), split_f16(v[q].z, vh[2], vl[2]), split_f16(v[q].w, vh[3], vl[3]);
+          mma16<false>(d, uh[0], vh[0], uh[1], vh[1], b[q].x, b[q].y);
+          mma16<false>(e, uh[2], vh[2], uh[3], vh[3], b[q].z, b[q].w);
+          mma16<false>(d, ul[0], vl[0], ul[1], vl[1], b[q].x, b[q].y);
+          mma16<false>(e, ul[2], vl[2], ul[3], vl[3], b[q].z, b[q].w);
+        } else {
+          mma16<false>(d, u[q].x, v[q].x, u[q].y, v[q].y, b[q].x, b[q].y);
+          mma16<false>(e, u[q].z, v[q].z, u[q].w, v[q].w, b[q].z, b[q].w);
+        }
       }
     }
     *reinterpret_cast<float2*>(&part[warp][g][2 * t]) = make_float2(d[0] + e[0], d[1] + e[1]);
     *reinterpret_cast<float2*>(&part[warp][g + 8][2 * t]) = make_float2(d[2] + e[2], d[3] + e[3]);
     __syncthreads();
     const int m = (int)threadIdx.x >> 3, j = threadIdx.x & 7;
-    if (m < rows && who[m] == ad) {
+    if (m < 16 && (mine >> m) & 1u) {
       float s = 0.f;
 #pragma unroll
       for (int q = 0; q < 8; ++q) s += part[q][m][j];
@@ -196,17 +201,6 @@ struct Shape {
 };
 static_assert(Shape<4>::bytes(MAX_K / 8) <= SMEM_MAX, "eight blocks hold the longest row");
 
-// Four fp32 numbers as pairs of bf16 numbers in three terms (eight bits each, the third rounded).
-DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
-  float4 r = v;
-#pragma unroll
-  for (int l = 0; l < 3; ++l) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(r.x, r.y), c = __floats2bfloat162_rn(r.z, r.w);
-    b0[l] = *reinterpret_cast<const uint32_t*>(&a), b1[l] = *reinterpret_cast<const uint32_t*>(&c);
-    r = make_float4(r.x - __low2float(a), r.y - __high2float(a), r.z - __low2float(c), r.w - __high2float(c));
-  }
-}
-
 // How a launch shares out its tiles and K: `each` tiles a cluster and one more for the first `more`; clusters of 1 << lcs blocks, 1 << lkw warps a
 // tile. All divisions are made on the host (a few dozen runtime divisions a thread took 3 us of 15).
 struct Split {
@@ -217,7 +211,7 @@ struct Split {
 template <bool F16, int NT>
 __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  int* who = reinterpret_cast<int*>(dyn);  // [8 NT] adapters of the pass's rows, then the different ones among them and their number
+  int* who = reinterpret_cast<int*>(dyn);  // adapters of the pass's rows
   unsigned char* xs = dyn + 256;
   float* sums = reinterpret_cast<float*>(xs + (size_t)8 * NT * sp.pitch);
   float* vs = sums + Shape<NT>::SUMS / 4;
@@ -293,22 +287,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
       }
     }
   }
-  int ndiff = 0;
-  if (p.rank > 0) {  // the different adapters, in every warp for itself
-    const unsigned same = __match_any_sync(0xffffffffu, ad);
-    const unsigned firsts = __ballot_sync(0xffffffffu, ad >= 0 && __ffs(same) - 1 == lane);
-    ndiff = __popc(firsts);
-    if (warp == 0) {
-      who[lane] = ad;
-      if ((firsts >> lane) & 1u) who[32 + __popc(firsts & ((1u << lane) - 1u))] = ad;
-    }
-  }
-  const bool tensor = ndiff > 0 && ndiff <= TENSOR_ADAPTERS && p.rows > TILE_ROWS;
-  // Without them: a warp takes the sixteen weight rows of a tile for a row of x, two lanes a weight row; the pairs of a batch are dealt out
+  const bool any = __ballot_sync(0xffffffffu, ad >= 0) != 0u;  // the same in every warp
+  if (warp == 0) who[lane] = ad;
+  // The adapters' second half: a warp takes the sixteen weight rows of a tile for a row of x, two lanes a weight row; the pairs of a batch are dealt out
   // over the cluster and its warps. The rows of B for the first batch come to L2 meanwhile.
   const int lr = lane >> 1, half = lane & 1;
   auto pair_row = [&](int tile, int a) { return p.b + ((size_t)a * p.n + min(16 * tile + lr, p.n - 1)) * p.rank; };
-  if (ndiff > 0 && !tensor)
+  if (any)
     for (int i = cr * CW + warp; i < min(tw, t1 - t0) * 8 * NT; i += cs * CW) {
       const int a = __shfl_sync(0xffffffffu, ad, i % (8 * NT));
       if (a >= 0 && 64 * half < p.rank) prefetch_line_l2(pair_row(t0 + i / (8 * NT), a) + 32 * half);
@@ -366,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
     }
     if (p.rank > 0 && bt == 0) {
       pdl_wait();  // v
-      if (ndiff > 0) {
+      if (any) {
         for (int i = threadIdx.x; i < 8 * NT * (MAX_RANK / 4); i += THREADS) {
           const int r = i / (MAX_RANK / 4), q = i % (MAX_RANK / 4);
           if (4 * q >= p.rank) continue;
@@ -374,29 +359,6 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
               r < cols && who[r] >= 0 ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         __syncthreads();
-      }
-    }
-    if (tensor && tile < t1) {
-      // B v as more inputs: sixteen ranks of an adapter at a time, dealt out over the K slices; rows of other adapters count as zeros
-#pragma unroll 1
-      for (int i0 = cr * kw + wk; i0 < ndiff * (MAX_RANK / 16); i0 += cs * kw) {
-        if (i0 % (MAX_RANK / 16) * 16 >= p.rank) continue;
-        const int ad = who[32 + i0 / (MAX_RANK / 16)], k0 = i0 % (MAX_RANK / 16) * 16 + 4 * t;
-        uint2 u = make_uint2(0u, 0u), v = u;
-        const bool in = k0 < p.rank;
-        if (in) {
-          u = __ldcg(reinterpret_cast<const uint2*>(p.b + ((size_t)ad * p.n + min(16 * tile + g, p.n - 1)) * p.rank + k0));
-          v = __ldcg(reinterpret_cast<const uint2*>(p.b + ((size_t)ad * p.n + min(16 * tile + g + 8, p.n - 1)) * p.rank + k0));
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (in && who[8 * i + g] == ad) f = *reinterpret_cast<const float4*>(vs + (8 * i + g) * (MAX_RANK + 4) + k0);
-          uint32_t q0[3], q1[3];
-          split3(f, q0, q1);
-#pragma unroll
-          for (int l = 2; l >= 0; --l) mma16<false>(acc[i], u.x, v.x, u.y, v.y, q0[l], q1[l]);
-        }
       }
     }
     __syncwarp();
@@ -408,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
       st[(8 * i + 2 * t) * PP + g + 8] = acc[i][2], st[(8 * i + 2 * t + 1) * PP + g + 8] = acc[i][3];
     }
     const int nt = min(tw, t1 - t0 - bt * tw);
-    if (ndiff > 0 && !tensor) {
+    if (any) {
       __syncthreads();
       constexpr int PAIRS = 8;  // on the way at once
       for (int i0 = cr * CW + warp; i0 < nt * 8 * NT; i0 += PAIRS * cs * CW) {

@@ -1,6 +1,6 @@
 // The projection of drb_proj_q8_lora for many rows: tcgen05 with the int8 codes handed over in tensor memory.
 //
-//   y [rows, n] = x W^T (+ res) + B v      D[128, nc] = W_tile[128, K] . x[nc, K]^T,  nc = 16 .. 96 rows of x
+//   y [rows, n] = x W^T (+ res) + B v      D[128, nc] = W_tile[128, K] . x[nc, K]^T,  nc = 16 .. 80 rows of x
 //
 // A code becomes a 16-bit number exactly, so the operand carries no scale: the multiplications of each 128 inputs have an
 // accumulator of their own (two, in turns), and the epilogue warps sum scale * accumulator in fp32 as they complete. An adapter of the
@@ -9,8 +9,8 @@
 // weight (bf16; fp16 one and a quarter) beside its loads and stores: 128 x 128 codes take a multiprocessor about 350 cycles, the
 // multiplications of nc = 80 take 160.
 //
-// Roles, one block of 14 warps per multiprocessor, meeting on mbarriers, every wait bounded: 8 convert warps (a thread 64 codes of one
-// weight row), 4 epilogue warps (a thread one weight row), one warp that issues the multiplications, one that issues the copies (tiled
+// Roles, one block of 14 warps per multiprocessor, meeting on mbarriers, every wait bounded: 8 convert warps (two sets that take turns; a
+// thread the 128 codes of one weight row), 4 epilogue warps (a thread one weight row), one warp that issues the multiplications, one that issues the copies (tiled
 // TMA, 128-byte swizzle). A block keeps its rows of x (blockIdx.y) and walks weight tiles.
 #pragma once
 
@@ -21,20 +21,20 @@ namespace pr {
 
 using namespace tc;
 
-constexpr int CONV = 8, EPI = 4, MMA_WARP = CONV + EPI, LOAD_WARP = MMA_WARP + 1, THREADS = (LOAD_WARP + 1) * 32;
+constexpr int CONV = 8, SET = 4, SETS = CONV / SET, EPI = 4, MMA_WARP = CONV + EPI, LOAD_WARP = MMA_WARP + 1, THREADS = (LOAD_WARP + 1) * 32;
 constexpr int NRAW = 4, NA = 3;            // raw stages of 16 KB; stages of A (64 columns of tensor memory) with a tile of x
-constexpr int MAX_C = 96;                  // rows of x a tile: their sums are an epilogue thread's registers
+constexpr int MAX_C = 80;                  // rows of x a tile: their sums are an epilogue thread's registers
 constexpr int RAW_BYTES = 128 * 128;
 constexpr int TMEM_COLS = 512, A_COL0 = 2 * MAX_C;
-static_assert(A_COL0 + NA * 64 <= TMEM_COLS, "tensor memory");
+static_assert(MAX_C == 80 && A_COL0 + NA * 64 <= TMEM_COLS, "tensor memory");
 
 struct Ctl {
-  uint64_t rawfull[NRAW], rawempty[NRAW];  // a raw stage has landed / has been read (one arrival per convert warp)
+  uint64_t rawfull[NRAW], rawempty[NRAW];  // a raw stage has landed / has been read (one arrival per convert warp of a set)
   uint64_t full[NA], done[NA];             // a stage is complete (convert warps, and the tile of x) / its multiplications have completed
   uint64_t accfull[2], accfree[2];         // an accumulator is complete / has been drained (one arrival per epilogue warp)
   uint32_t tmem;
   unsigned firsts[3];
-  __align__(16) int who[MAX_C];            // adapters of the tile's rows, -1: none
+  __align__(16) int who[96];            // adapters of the tile's rows, -1: none
   int diff[MAX_C];                         // the different ones among them
 };
 constexpr int CTL_BYTES = 1024;
@@ -46,6 +46,17 @@ static size_t smem_bytes(int nc) { return 1024 + CTL_BYTES + NRAW * RAW_BYTES + 
 struct Maps {
   CUtensorMap w, x;
 };
+
+// Four fp32 numbers as pairs of bf16 numbers in three terms (eight bits each, the third rounded).
+DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
+  float4 r = v;
+#pragma unroll
+  for (int l = 0; l < 3; ++l) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(r.x, r.y), c = __floats2bfloat162_rn(r.z, r.w);
+    b0[l] = *reinterpret_cast<const uint32_t*>(&a), b1[l] = *reinterpret_cast<const uint32_t*>(&c);
+    r = make_float4(r.x - __low2float(a), r.y - __high2float(a), r.z - __low2float(c), r.w - __high2float(c));
+  }
+}
 
 template <bool F16>
 __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant__ Maps maps, pl::Args p, int nc, int tiles) {
@@ -73,8 +84,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
   const int nw = mine * groups;
   if (warp == LOAD_WARP) {
     if (elect_one()) {
-      for (int s = 0; s < NRAW; ++s) mbar_init(&ctl.rawfull[s], 1), mbar_init(&ctl.rawempty[s], CONV);
-      for (int s = 0; s < NA; ++s) mbar_init(&ctl.full[s], CONV + 1), mbar_init(&ctl.done[s], 1);
+      for (int s = 0; s < NRAW; ++s) mbar_init(&ctl.rawfull[s], 1), mbar_init(&ctl.rawempty[s], SET);
+      for (int s = 0; s < NA; ++s) mbar_init(&ctl.full[s], SET + 1), mbar_init(&ctl.done[s], 1);
       for (int s = 0; s < 2; ++s) mbar_init(&ctl.accfull[s], 1), mbar_init(&ctl.accfree[s], EPI);
       mbar_fence_init();
       while (wi < NRAW && wi < nw) load_w();
@@ -85,80 +96,99 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
   pdl_launch_dependents();
   // The tile's adapters and the different ones among them. With adapters x and adapter_of are older than the launch before (see proj_lora.cuh).
   const int a = p.rank > 0 && (int)threadIdx.x < cols ? pl::adapter(p, row0 + threadIdx.x) : -1;
-  if (threadIdx.x < MAX_C) ctl.who[threadIdx.x] = a;
+  if (threadIdx.x < 96) ctl.who[threadIdx.x] = a;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl.tmem;
   int ndiff = 0;
   if (p.rank > 0) {
-    if (threadIdx.x < MAX_C) {
+    if (threadIdx.x < 96) {
       bool is_first = a >= 0;
-      for (int j = 0; j < (int)threadIdx.x; ++j) is_first = is_first && ctl.who[j] != a;
+#pragma unroll 8
+      for (int j = 0; j < (int)threadIdx.x; j += 4) {
+        const int4 w = *reinterpret_cast<const int4*>(&ctl.who[j]);
+        const int left = (int)threadIdx.x - j;
+        is_first = is_first && w.x != a && !(left > 1 && w.y == a) && !(left > 2 && w.z == a) && !(left > 3 && w.w == a);
+      }
       const unsigned f = __ballot_sync(0xffffffffu, is_first);
       if (lane == 0) ctl.firsts[warp] = f;
     }
     __syncthreads();
     const unsigned f0 = ctl.firsts[0], f1 = ctl.firsts[1], f2 = ctl.firsts[2];
     ndiff = __popc(f0) + __popc(f1) + __popc(f2);
-    if (threadIdx.x < MAX_C && (ctl.firsts[warp] >> lane) & 1u)
+    if (threadIdx.x < 96 && (ctl.firsts[warp] >> lane) & 1u)
       ctl.diff[(warp > 0 ? __popc(f0) : 0) + (warp > 1 ? __popc(f1) : 0) + __popc(ctl.firsts[warp] & ((1u << lane) - 1u))] = a;
     __syncthreads();
   }
   const int seq = groups + ndiff, total = mine * seq;  // stretches of inputs: a tile's 128s, then its adapters
 
   if (warp < CONV) {
-    // ---------------- convert: warp w takes lanes 32 (w % 4) .. of the tile and the inputs 64 (w / 4) .. of a stretch
-    const int q = warp & 3, half = warp >> 2, row = 32 * q + lane;
-    const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + A_COL0 + 32 * half;
+    // ---------------- convert: two sets of four warps take turns at the stretches; a thread has one row of the tile
+    const int q = warp & 3, row = 32 * q + lane;
+    const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + A_COL0;
     bool awaited = false;
-    int cw = 0;
-    for (int c = 0, t = 0, g = 0; c < total; ++c) {
+    for (int c = warp >> 2, t = c / seq, g = c % seq; c < total; c += SETS) {
       const int s = c % NA, use = c / NA;
       uint32_t o[32];
       if (g < groups) {
-        const int r = cw % NRAW;
+        const int cw = t * groups + g, r = cw % NRAW;
         mbar_wait_ring<DRB_ERR_FULL_WAIT>(smem_u32(&ctl.rawfull[r]), (cw / NRAW) & 1, spent);
-        ++cw;
-        uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(raw + r * RAW_BYTES + swz_off(row, 4 * half + j));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.rawempty[r]);
+        for (int half = 0; half < 2; ++half) {
+          uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          pl::widen_codes<F16>(v[j].x, o[8 * j], o[8 * j + 1]);
-          pl::widen_codes<F16>(v[j].y, o[8 * j + 2], o[8 * j + 3]);
-          pl::widen_codes<F16>(v[j].z, o[8 * j + 4], o[8 * j + 5]);
-          pl::widen_codes<F16>(v[j].w, o[8 * j + 6], o[8 * j + 7]);
+          for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(raw + r * RAW_BYTES + swz_off(row, 4 * half + j));
+          if (half == 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.rawempty[r]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            pl::widen_codes<F16>(v[j].x, o[8 * j], o[8 * j + 1]);
+            pl::widen_codes<F16>(v[j].y, o[8 * j + 2], o[8 * j + 3]);
+            pl::widen_codes<F16>(v[j].z, o[8 * j + 4], o[8 * j + 5]);
+            pl::widen_codes<F16>(v[j].w, o[8 * j + 6], o[8 * j + 7]);
+          }
+          if (half == 0) {
+            if (use > 0) mbar_wait_ring<DRB_ERR_TMEM>(smem_u32(&ctl.done[s]), (use - 1) & 1, spent);
+            tc_fence_after();
+          }
+          tmem_st32(ta + 64 * s + 32 * half, o);
+        }
+      } else {
+        // an adapter: 64 ranks (zeros behind the last) of B's rows, and v
+        const int ad = ctl.diff[g - groups], wr = (first + t * step) * 128 + row;
+        const uint4* bp = reinterpret_cast<const uint4*>(p.b + ((size_t)ad * p.n + min(wr, p.n - 1)) * p.rank);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint4 b = 8 * j < p.rank ? __ldcg(bp + j) : make_uint4(0u, 0u, 0u, 0u);
+          o[4 * j] = b.x, o[4 * j + 1] = b.y, o[4 * j + 2] = b.z, o[4 * j + 3] = b.w;
         }
         if (use > 0) mbar_wait_ring<DRB_ERR_TMEM>(smem_u32(&ctl.done[s]), (use - 1) & 1, spent);
         tc_fence_after();
         tmem_st32(ta + 64 * s, o);
-      } else {
-        // an adapter: 64 ranks (zeros behind the last) of B's rows, and v
         if (!awaited) pdl_wait(), awaited = true;
-        if (use > 0) mbar_wait_ring<DRB_ERR_TMEM>(smem_u32(&ctl.done[s]), (use - 1) & 1, spent);
-        tc_fence_after();
-        const int ad = ctl.diff[g - groups], wr = (first + t * step) * 128 + row;
-        if (half == 0) {
-          const uint4* bp = reinterpret_cast<const uint4*>(p.b + ((size_t)ad * p.n + min(wr, p.n - 1)) * p.rank);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint4 b = 8 * j < p.rank ? __ldcg(bp + j) : make_uint4(0u, 0u, 0u, 0u);
-            o[4 * j] = b.x, o[4 * j + 1] = b.y, o[4 * j + 2] = b.z, o[4 * j + 3] = b.w;
-          }
-          tmem_st32(ta + 64 * s, o);
-        }
         unsigned char* xs = xst + s * xstage;
-        for (int i = threadIdx.x; i < nc * 16; i += CONV * 32) {  // four ranks of a row
-          const int r = i >> 4, k4 = i & 15;
-          const float4 f = ctl.who[r] == ad && 4 * k4 < p.rank ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + k4)
-                                                               : make_float4(0.f, 0.f, 0.f, 0.f);
-          uint32_t b0[3], b1[3];
-          pl::split3(f, b0, b1);
+        // four ranks of a row a thread, five rows at once: thread i takes ranks 4 (i % 16) .. of rows i / 16, i / 16 + 8, ...
+        const int k4 = threadIdx.x & 15;
+        for (int r0 = (threadIdx.x & (SET * 32 - 1)) >> 4; r0 < nc; r0 += 40) {
+          float4 f[5];
 #pragma unroll
-          for (int l = 0; l < 3; ++l) *reinterpret_cast<uint2*>(xs + l * box + swz_off(r, k4 >> 1) + 8 * (k4 & 1)) = make_uint2(b0[l], b1[l]);
+          for (int i = 0; i < 5; ++i) {
+            const int r = r0 + 8 * i;
+            f[i] = r < nc && ctl.who[r] == ad && 4 * k4 < p.rank ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + k4)
+                                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int i = 0; i < 5; ++i) {
+            const int r = r0 + 8 * i;
+            if (r >= nc) break;
+            uint32_t b0[3], b1[3];
+            split3(f[i], b0, b1);
+#pragma unroll
+            for (int l = 0; l < 3; ++l) *reinterpret_cast<uint2*>(xs + l * box + swz_off(r, k4 >> 1) + 8 * (k4 & 1)) = make_uint2(b0[l], b1[l]);
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the multiplications read v through the asynchronous proxy
       }
@@ -166,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.full[s]);
-      if (++g == seq) g = 0, ++t;
+      for (g += SETS; g >= seq; g -= seq) ++t;
     }
     if (!awaited) pdl_wait();  // this launch never ends before the one that it follows
   } else if (warp < MMA_WARP) {
@@ -189,17 +219,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
       mbar_wait_ring<DRB_ERR_TMEM>(smem_u32(&ctl.accfull[c & 1]), (c >> 1) & 1, spent);
       tc_fence_after();
       const float f = __half2float(h);
+      // columns behind nc hold anything and are not stored
+      const uint32_t at = td + (c & 1) * MAX_C;
+      auto drained = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.accfree[c & 1]);
+      };
 #pragma unroll
-      for (int j = 0; j < MAX_C / 16; ++j)
-        if (16 * j < nc) {
-          uint32_t d[16];
-          tmem_ld16(td + (c & 1) * MAX_C + 16 * j, d);
+      for (int j = 0; j < 2; ++j)
+        if (32 * j < nc) {
+          uint32_t d[32];
+          tmem_ld32(at + 32 * j, d);
+          if (32 * (j + 1) >= nc) drained();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[16 * j + e] = fmaf(f, __uint_as_float(d[e]), acc[16 * j + e]);
+          for (int e = 0; e < 32; ++e) acc[32 * j + e] = fmaf(f, __uint_as_float(d[e]), acc[32 * j + e]);
         }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.accfree[c & 1]);
+      if (nc > 64) {
+        uint32_t d[16];
+        tmem_ld16(at + 64, d);
+        drained();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[64 + e] = fmaf(f, __uint_as_float(d[e]), acc[64 + e]);
+      }
       if (++g == seq) {
         g = 0;
         if (o < p.n) {
@@ -210,10 +252,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
             if (j >= cols) break;
             float add[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) add[e] = res && j + e < cols ? __ldcg(res + (size_t)(j + e) * p.n) : 0.f;
+            for (int e = 0; e < 8; ++e) {
+              add[e] = res && j + e < cols ? __ldcg(res) : 0.f;
+              if (res) res += p.n;
+            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (j + e < cols) y[(size_t)(j + e) * p.n] = acc[j + e] + add[e];
+            for (int e = 0; e < 8; ++e, y += p.n)
+              if (j + e < cols) *y = acc[j + e] + add[e];
           }
         }
       }
@@ -274,7 +319,7 @@ static int map_2d(CUtensorMap* m, CUtensorMapDataType type, const void* p, uint6
   return pft::encode(m, type, 2, p, dims, strides, box);
 }
 
-// As few passes over the weights as tiles of up to 96 rows of x allow, equally wide.
+// As few passes over the weights as tiles of up to 80 rows of x allow, equally wide.
 template <bool F16>
 static int launch(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
   const int ny = (p.rows + MAX_C - 1) / MAX_C, nc = ((p.rows + ny - 1) / ny + 15) / 16 * 16, passes = (p.rows + nc - 1) / nc;
