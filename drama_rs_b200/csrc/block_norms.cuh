@@ -9,12 +9,14 @@
 // beside o and h), by the launch and two block-wide sums for few.
 #pragma once
 
-#include "common.cuh"
+#include <type_traits>
 
+#include "common.cuh"
 
 namespace bn {
 
-constexpr int MAX_D = 8192;  // eight values a thread
+constexpr int MAX_D = 8192;  // sixteen values a thread
+constexpr int BLOCKS = 5;    // of 128 threads a multiprocessor
 enum Type { F32 = 0, BF16 = 1, F16 = 2 };
 
 struct Args {
@@ -22,145 +24,170 @@ struct Args {
   const float *post_w, *gate, *scale, *x, *pre_w;
   float* x_out;
   void* h;
-  int o_type, h_type, d;
+  int d;
   float alpha, eps;
 };
 
 DRB_DEV float clamp_f16(float v) { return v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v; }  // a NaN stays one
 
-DRB_DEV float widen(uint16_t b, int type) {
-  return type == BF16 ? __uint_as_float((uint32_t)b << 16) : __half2float(__ushort_as_half(b));
+template <int TYPE>
+DRB_DEV float2 widen(uint32_t w) {
+  return TYPE == BF16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-DRB_DEV uint16_t narrow(float v, int type) {
-  return type == BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(clamp_f16(v)));
+template <int TYPE>
+DRB_DEV uint32_t narrow(float lo, float hi) {
+  if (TYPE == BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(clamp_f16(lo), clamp_f16(hi));
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The block's sum of v in every thread; `red` holds one value per warp and is used once.
+// The block's sum of v in every thread: butterfly, then the warps in fours. `red` is one value per warp, zeros behind the last.
 DRB_DEV float block_sum(float v, float* red) {
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   float s = 0.f;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += red[w];
+  for (int w = 0; w < (int)blockDim.x; w += 128) {
+    const float4 q = *reinterpret_cast<const float4*>(red + (w >> 5));
+    s += (q.x + q.y) + (q.z + q.w);
+  }
   return s;
 }
 
-// Eight values of a row a thread: eight consecutive ones (WIDE: 16-byte accesses, d a multiple of 8 and every pointer aligned), or every
-// blockDim-th one for any other row. A block keeps its part of the weights in registers and goes through rows blockIdx, + gridDim, ...; the
-// next row is requested before the current one's sums, so that the stream does not wait for them.
+// Sixteen values of a row a thread: four times four consecutive ones (WIDE: 16- and 8-byte accesses next to one another, d a multiple of 4 and
+// every pointer aligned), or every blockDim-th one for any other row. A block keeps its part of the weights in registers and goes
+// through rows blockIdx, + gridDim, ...; the next row is requested before the current one's sums, so that the stream does not wait for
+// them. (Eight values a thread took two thirds longer over the sums: as many shuffles and barriers for half the values.)
+constexpr int V = 16;
 template <bool WIDE>
 struct Cols {
   int c0, step, d;
-  DRB_DEV Cols(int d) : c0(threadIdx.x * (WIDE ? 8 : 1)), step(WIDE ? 1 : blockDim.x), d(d) {}
-  DRB_DEV bool in(int j) const { return WIDE ? c0 < d : c0 + j * step < d; }
-  DRB_DEV void load(const float* p, float (&v)[8]) const {
+  DRB_DEV Cols(int d) : c0(threadIdx.x * (WIDE ? 4 : 1)), step(blockDim.x * (WIDE ? 4 : 1)), d(d) {}
+  // value j lies in column at(j); WIDE: values 4 i .. 4 i + 3 are in the row together
+  DRB_DEV int at(int j) const { return WIDE ? c0 + (j >> 2) * step + (j & 3) : c0 + j * step; }
+  DRB_DEV bool in(int j) const { return at(j) < d; }
+  DRB_DEV void load(const float* p, float (&v)[V]) const {
     if constexpr (WIDE) {
-      if (!in(0)) return;
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(p + c0)), b = __ldcg(reinterpret_cast<const float4*>(p + c0) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+#pragma unroll
+      for (int j = 0; j < V; j += 4)
+        if (in(j)) {
+          const float4 a = __ldcg(reinterpret_cast<const float4*>(p + at(j)));
+          v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
+        }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (in(j)) v[j] = __ldcg(p + c0 + j * step);
+      for (int j = 0; j < V; ++j)
+        if (in(j)) v[j] = __ldcg(p + at(j));
     }
   }
-  DRB_DEV void store(float* p, const float (&v)[8]) const {
+  DRB_DEV void store(float* p, const float (&v)[V]) const {
     if constexpr (WIDE) {
-      if (!in(0)) return;
-      reinterpret_cast<float4*>(p + c0)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p + c0)[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+      for (int j = 0; j < V; j += 4)
+        if (in(j)) *reinterpret_cast<float4*>(p + at(j)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (in(j)) p[c0 + j * step] = v[j];
+      for (int j = 0; j < V; ++j)
+        if (in(j)) p[at(j)] = v[j];
     }
   }
   // 16-bit values stay as they are until they are used: w[j] holds values 2 j and 2 j + 1
-  DRB_DEV void load16(const uint16_t* p, uint32_t (&w)[4]) const {
+  DRB_DEV void load16(const uint16_t* p, uint32_t (&w)[V / 2]) const {
     if constexpr (WIDE) {
-      if (!in(0)) return;
-      const uint4 a = __ldcg(reinterpret_cast<const uint4*>(p + c0));
-      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+#pragma unroll
+      for (int j = 0; j < V; j += 4)
+        if (in(j)) {
+          const uint2 a = __ldcg(reinterpret_cast<const uint2*>(p + at(j)));
+          w[j / 2] = a.x, w[j / 2 + 1] = a.y;
+        }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = in(2 * j) ? __ldcg(p + c0 + 2 * j * step) : 0u, hi = in(2 * j + 1) ? __ldcg(p + c0 + (2 * j + 1) * step) : 0u;
+      for (int j = 0; j < V / 2; ++j) {
+        const uint32_t lo = in(2 * j) ? __ldcg(p + at(2 * j)) : 0u, hi = in(2 * j + 1) ? __ldcg(p + at(2 * j + 1)) : 0u;
         w[j] = lo | hi << 16;
       }
     }
   }
-  DRB_DEV void store16(uint16_t* p, const float (&v)[8], int type) const {
+  template <int TYPE>
+  DRB_DEV void store16(uint16_t* p, const float (&v)[V]) const {
     if constexpr (WIDE) {
-      if (!in(0)) return;
-      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = (uint32_t)narrow(v[2 * j], type) | (uint32_t)narrow(v[2 * j + 1], type) << 16;
-      *reinterpret_cast<uint4*>(p + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int j = 0; j < V; j += 4)
+        if (in(j)) *reinterpret_cast<uint2*>(p + at(j)) = make_uint2(narrow<TYPE>(v[j], v[j + 1]), narrow<TYPE>(v[j + 2], v[j + 3]));
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (in(j)) p[c0 + j * step] = narrow(v[j], type);
+      for (int j = 0; j < V; j += 2) {
+        const uint32_t w = narrow<TYPE>(v[j], v[j + 1]);
+        if (in(j)) p[at(j)] = (uint16_t)w;
+        if (in(j + 1)) p[at(j + 1)] = (uint16_t)(w >> 16);
+      }
     }
   }
 };
 
-template <bool WIDE, bool O16, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1) k_block_norms(Args a, int rows) {
-  __shared__ float red[2][32];
+template <bool WIDE, int OT, int HT, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 128 ? BLOCKS : 1) k_block_norms(Args a, int rows) {
+  __shared__ __align__(16) float red[2][32];
   const int d = a.d;
   const Cols<WIDE> cols(d);
+  if (threadIdx.x < 64) red[0][threadIdx.x] = 0.f;  // a block has 32 threads at least
+  if (blockDim.x == 32) red[1][threadIdx.x] = 0.f;
+  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
-  float xn[8] = {}, on[8] = {}, gn = 0.f;
-  uint32_t hn[4] = {};
+  float xn[V] = {}, on[V] = {}, gn = 0.f;
+  uint32_t hn[V / 2] = {};
   auto fetch = [&](int row) {
     const size_t at = (size_t)row * d;
     cols.load(a.x + at, xn);
-    if constexpr (O16) cols.load16(static_cast<const uint16_t*>(a.o) + at, hn);
+    if constexpr (OT != F32) cols.load16(static_cast<const uint16_t*>(a.o) + at, hn);
     else cols.load(static_cast<const float*>(a.o) + at, on);
     if (a.gate) gn = __ldcg(a.gate + row);
   };
   fetch(blockIdx.x);
-  float wt[8], wn[8] = {};  // post_w * scale, pre_w
+  float wt[V], wn[V] = {};  // post_w * scale, pre_w
   {
-    float w[8], s[8];
+    float w[V], s[V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = s[j] = 1.f;
+    for (int j = 0; j < V; ++j) w[j] = s[j] = 1.f;
     if (a.post_w) cols.load(a.post_w, w);
     if (a.scale) cols.load(a.scale, s);
     if (a.pre_w) cols.load(a.pre_w, wn);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) wt[j] = w[j] * s[j];
+    for (int j = 0; j < V; ++j) wt[j] = w[j] * s[j];
   }
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const size_t at = (size_t)row * d;
-    float x[8], t[8];
+    float x[V], t[V];
     const float gate = gn;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = xn[j];
-      if constexpr (O16) t[j] = widen((uint16_t)(hn[j / 2] >> (j & 1 ? 16 : 0)), a.o_type);
-      else t[j] = on[j];
+    for (int j = 0; j < V; j += 2) {
+      x[j] = xn[j], x[j + 1] = xn[j + 1];
+      const float2 v = OT == F32 ? make_float2(on[j], on[j + 1]) : widen<OT>(hn[j / 2]);
+      t[j] = v.x, t[j + 1] = v.y;
     }
     if (row + (int)gridDim.x < rows) fetch(row + gridDim.x);
     float f = 1.f;
     if (a.post_w) {
       float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(t[j], t[j], ss);
+      for (int j = 0; j < V; ++j) ss = fmaf(t[j], t[j], ss);
       f = rsqrtf(block_sum(ss, red[0]) / (float)d + a.eps);
     }
     if (a.gate) f *= sigmoid_f(gate);
     float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = fmaf(f, t[j] * wt[j], a.alpha * x[j]), ss = fmaf(x[j], x[j], ss);
+    for (int j = 0; j < V; ++j) x[j] = fmaf(f, t[j] * wt[j], a.alpha * x[j]), ss = fmaf(x[j], x[j], ss);
     cols.store(a.x_out + at, x);
     if (a.pre_w) {
       const float r = rsqrtf(block_sum(ss, red[1]) / (float)d + a.eps);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * r * wn[j];
-      if (a.h_type == F32) cols.store(static_cast<float*>(a.h) + at, x);
-      else cols.store16(static_cast<uint16_t*>(a.h) + at, x, a.h_type);
+      for (int j = 0; j < V; ++j) x[j] = x[j] * r * wn[j];
+      if constexpr (HT == F32) cols.store(static_cast<float*>(a.h) + at, x);
+      else cols.template store16<HT>(static_cast<uint16_t*>(a.h) + at, x);
     }
     // a warp writes its slot of one sum again only behind the other sum's barrier; with one sum a row it has to be kept apart
     if (!a.post_w || !a.pre_w) __syncthreads();
@@ -168,33 +195,46 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 3 : 1) k_block_norms(Args 
 }
 
 // As many blocks as are resident at once go through the rows together.
-template <bool WIDE, bool O16, int MAXT>
+template <bool WIDE, int OT, int HT, int MAXT>
 static void launch(const Args& a, int rows, cudaStream_t st, const DrbDevice& dev) {
-  const int threads = ((a.d + 7) / 8 + 31) / 32 * 32;
-  const int fit = dev.sms * (MAXT == 256 ? 768 / threads : 1);
-  drb_launch(k_block_norms<WIDE, O16, MAXT>, dim3(rows < fit ? rows : fit), dim3(threads), 0, st, dev.pdl, a, rows);
+  const int threads = ((a.d + V - 1) / V + 31) / 32 * 32;
+  const int fit = dev.sms * (MAXT == 128 ? BLOCKS * 128 / threads : 1);
+  drb_launch(k_block_norms<WIDE, OT, HT, MAXT>, dim3(rows < fit ? rows : fit), dim3(threads), 0, st, dev.pdl, a, rows);
 }
 
-template <bool WIDE, bool O16>
-static void launch_any(const Args& a, int rows, cudaStream_t st, const DrbDevice& dev) {
-  if (a.d <= 2048) launch<WIDE, O16, 256>(a, rows, st, dev);
-  else if (a.d <= 4096) launch<WIDE, O16, 512>(a, rows, st, dev);
-  else launch<WIDE, O16, 1024>(a, rows, st, dev);
+// The kernels for every pair of types, as one list for launches and set-up.
+template <typename F>
+static auto for_types(int o_type, int h_type, F f) {
+  using std::integral_constant;
+  const auto inner = [&](auto o) {
+    return h_type == F32 ? f(o, integral_constant<int, F32>()) : h_type == BF16 ? f(o, integral_constant<int, BF16>()) : f(o, integral_constant<int, F16>());
+  };
+  return o_type == F32 ? inner(integral_constant<int, F32>()) : o_type == BF16 ? inner(integral_constant<int, BF16>()) : inner(integral_constant<int, F16>());
 }
 
-template <bool WIDE, bool O16>
-static cudaError_t configure() {
-  cudaError_t e;
-  if ((e = drb_carveout(k_block_norms<WIDE, O16, 256>)) != cudaSuccess) return e;
-  if ((e = drb_carveout(k_block_norms<WIDE, O16, 512>)) != cudaSuccess) return e;
-  return drb_carveout(k_block_norms<WIDE, O16, 1024>);
+static void launch_any(bool wide, const Args& a, int o_type, int h_type, int rows, cudaStream_t st, const DrbDevice& dev) {
+  for_types(o_type, h_type, [&](auto o, auto h) {
+    constexpr int OT = decltype(o)::value, HT = decltype(h)::value;
+    if (wide) a.d <= 2048 ? launch<true, OT, HT, 128>(a, rows, st, dev) : launch<true, OT, HT, 512>(a, rows, st, dev);
+    else a.d <= 2048 ? launch<false, OT, HT, 128>(a, rows, st, dev) : launch<false, OT, HT, 512>(a, rows, st, dev);
+    return 0;
+  });
 }
+
 static cudaError_t configure_all() {
-  cudaError_t e;
-  if ((e = configure<true, true>()) != cudaSuccess) return e;
-  if ((e = configure<true, false>()) != cudaSuccess) return e;
-  if ((e = configure<false, true>()) != cudaSuccess) return e;
-  return configure<false, false>();
+  for (int o = 0; o < 3; ++o)
+    for (int h = 0; h < 3; ++h) {
+      const cudaError_t e = for_types(o, h, [](auto ot, auto ht) {
+        constexpr int OT = decltype(ot)::value, HT = decltype(ht)::value;
+        cudaError_t e;
+        if ((e = drb_carveout(k_block_norms<true, OT, HT, 128>)) != cudaSuccess) return e;
+        if ((e = drb_carveout(k_block_norms<true, OT, HT, 512>)) != cudaSuccess) return e;
+        if ((e = drb_carveout(k_block_norms<false, OT, HT, 128>)) != cudaSuccess) return e;
+        return drb_carveout(k_block_norms<false, OT, HT, 512>);
+      });
+      if (e != cudaSuccess) return e;
+    }
+  return cudaSuccess;
 }
 
 }  // namespace bn
@@ -209,9 +249,8 @@ extern "C" int drb_block_norms(const void* o, int o_type, const float* post_w, c
   const DrbDevice& dev = drb_device(st);
   if (!dev.ready) return -2;
   if (rows == 0) return 0;
-  const bn::Args a = {o, post_w, gate, scale, x, pre_w, x_out, h, o_type, h_type, d, alpha, eps};
-  const bool wide = d % 8 == 0 && !off(o, 16) && !off(x, 16) && !off(x_out, 16) && !off(post_w, 16) && !off(scale, 16) && !off(pre_w, 16) && !(pre_w && off(h, 16));
-  if (wide) o_type ? bn::launch_any<true, true>(a, rows, st, dev) : bn::launch_any<true, false>(a, rows, st, dev);
-  else o_type ? bn::launch_any<false, true>(a, rows, st, dev) : bn::launch_any<false, false>(a, rows, st, dev);
+  const bn::Args a = {o, post_w, gate, scale, x, pre_w, x_out, h, d, alpha, eps};
+  const bool wide = d % 4 == 0 && !off(o, o_type ? 8 : 16) && !off(x, 16) && !off(x_out, 16) && !off(post_w, 16) && !off(scale, 16) && !off(pre_w, 16) && !(pre_w && off(h, h_type ? 8 : 16));
+  bn::launch_any(wide, a, o_type, h_type, rows, st, dev);
   return 0;
 }

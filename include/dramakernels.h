@@ -323,7 +323,7 @@ int drb_proj_q8_lora(const int8_t* w, const dr_half* s, const void* x, int x_typ
  *   scale [d]: NULL = 1); h = rmsnorm(x_out, pre_w, eps) (pre_w NULL: no h is written and h may be NULL).
  * o of o_type and h of h_type (DRB_F32, DRB_BF16, DRB_F16; an fp16 h is clamped to +-65504, a NaN stays one), everything else f32. Sums in
  * fp32; a row's result does not depend on the number of rows. x_out may be x, and h may be o when their types are of one size.
- * 1 <= d <= 8192, else -1; any alignment of a value's own size (-3 otherwise), 16-byte aligned buffers and d % 8 == 0 are fastest.
+ * 1 <= d <= 8192, else -1; any alignment of a value's own size (-3 otherwise), 16-byte aligned buffers and d % 4 == 0 are fastest.
  * All operands, weights too, may be the work of the launch before. */
 int drb_block_norms(const void* o, int o_type, const float* post_w, const float* gate, const float* scale, float alpha, const float* x,
                     float* x_out, const float* pre_w, void* h, int h_type, int rows, int d, float eps, dr_stream st);
