@@ -17,6 +17,8 @@ namespace bn {
 
 constexpr int MAX_D = 8192;  // sixteen values a thread
 constexpr int BLOCKS = 5;    // of 128 threads a multiprocessor
+constexpr int depth(int maxt) { return maxt == 128 ? 4 : 3; }  // rows under way and in use
+constexpr int SMEM_MAX = 220 * 1024;  // of a multiprocessor, beside what the system takes of it
 enum Type { F32 = 0, BF16 = 1, F16 = 2 };
 
 struct Args {
@@ -59,8 +61,8 @@ DRB_DEV float block_sum(float v, float* red) {
 
 // Sixteen values of a row a thread: four times four consecutive ones (WIDE: 16- and 8-byte accesses next to one another, d a multiple of 4 and
 // every pointer aligned), or every blockDim-th one for any other row. A block keeps its part of the weights in registers and goes
-// through rows blockIdx, + gridDim, ...; the next row is requested before the current one's sums, so that the stream does not wait for
-// them. (Eight values a thread took two thirds longer over the sums: as many shuffles and barriers for half the values.)
+// through rows blockIdx, + gridDim, ...; the next rows (WIDE: three, through shared memory; else one, in registers) are requested before the
+// current one's sums, so that the stream does not wait for them. (Eight values a thread took two thirds longer over the sums: as many shuffles and barriers for half the values.)
 constexpr int V = 16;
 template <bool WIDE>
 struct Cols {
@@ -131,6 +133,8 @@ struct Cols {
 template <bool WIDE, int OT, int HT, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 128 ? BLOCKS : 1) k_block_norms(Args a, int rows) {
   __shared__ __align__(16) float red[2][32];
+  constexpr int OSIZE = OT == F32 ? 16 : 8;  // bytes of four values of o
+  constexpr int DEPTH = MAXT == 128 ? 4 : 3;
   const int d = a.d;
   const Cols<WIDE> cols(d);
   if (threadIdx.x < 64) red[0][threadIdx.x] = 0.f;  // a block has 32 threads at least
@@ -138,16 +142,41 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? BLOCKS : 1) k_block_norms(
   __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
-  float xn[V] = {}, on[V] = {}, gn = 0.f;
+  float xn[V] = {}, on[V] = {}, gn = 0.f;  // !WIDE: the next row
   uint32_t hn[V / 2] = {};
+  extern __shared__ __align__(16) unsigned char ring[];
   auto fetch = [&](int row) {
     const size_t at = (size_t)row * d;
     cols.load(a.x + at, xn);
     if constexpr (OT != F32) cols.load16(static_cast<const uint16_t*>(a.o) + at, hn);
     else cols.load(static_cast<const float*>(a.o) + at, on);
-    if (a.gate) gn = __ldcg(a.gate + row);
   };
-  fetch(blockIdx.x);
+  // WIDE: rows on their way into DEPTH slots of shared memory, where every thread finds what it copied itself: no barrier, no registers
+  const uint32_t slots = smem_u32(ring) + 16 * threadIdx.x, pitch = 16 * blockDim.x, oslots = smem_u32(ring) + 4 * pitch + OSIZE * threadIdx.x;
+  const uint32_t opitch = OSIZE * blockDim.x, slot_bytes = 4 * (pitch + opitch);
+  auto request = [&](int row, int slot) {
+    if (row < rows) {
+      const float* x = a.x + (size_t)row * d;
+      const unsigned char* o = static_cast<const unsigned char*>(a.o) + (size_t)row * d * (OSIZE / 4);
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        if (cols.in(4 * i)) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + slot * slot_bytes + i * pitch), "l"(x + cols.at(4 * i)) : "memory");
+          if constexpr (OT == F32)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(oslots + slot * slot_bytes + i * opitch), "l"(o + 4 * (size_t)cols.at(4 * i)) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(oslots + slot * slot_bytes + i * opitch), "l"(o + 2 * (size_t)cols.at(4 * i)) : "memory");
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int k = 0; k < DEPTH - 1; ++k) request(blockIdx.x + k * gridDim.x, k);
+  } else {
+    fetch(blockIdx.x);
+  }
+  if (a.gate) gn = __ldcg(a.gate + blockIdx.x);
   float wt[V], wn[V] = {};  // post_w * scale, pre_w
   {
     float w[V], s[V];
@@ -159,17 +188,43 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? BLOCKS : 1) k_block_norms(
 #pragma unroll
     for (int j = 0; j < V; ++j) wt[j] = w[j] * s[j];
   }
+  int slot = 0;
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const size_t at = (size_t)row * d;
     float x[V], t[V];
     const float gate = gn;
+    const bool more = row + (int)gridDim.x < rows;
+    if (a.gate && more) gn = __ldcg(a.gate + row + gridDim.x);
+    if constexpr (WIDE) {
+      request(row + (DEPTH - 1) * gridDim.x, slot == 0 ? DEPTH - 1 : slot - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
 #pragma unroll
-    for (int j = 0; j < V; j += 2) {
-      x[j] = xn[j], x[j + 1] = xn[j + 1];
-      const float2 v = OT == F32 ? make_float2(on[j], on[j + 1]) : widen<OT>(hn[j / 2]);
-      t[j] = v.x, t[j + 1] = v.y;
+      for (int i = 0; i < V / 4; ++i) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+        if (cols.in(4 * i)) {
+          v = *static_cast<const float4*>(__cvta_shared_to_generic(slots + slot * slot_bytes + i * pitch));
+          const uint32_t q = oslots + slot * slot_bytes + i * opitch;
+          if constexpr (OT == F32) {
+            u = *static_cast<const float4*>(__cvta_shared_to_generic(q));
+          } else {
+            const uint2 w = *static_cast<const uint2*>(__cvta_shared_to_generic(q));
+            const float2 lo = widen<OT>(w.x), hi = widen<OT>(w.y);
+            u = make_float4(lo.x, lo.y, hi.x, hi.y);
+          }
+        }
+        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        t[4 * i] = u.x, t[4 * i + 1] = u.y, t[4 * i + 2] = u.z, t[4 * i + 3] = u.w;
+      }
+      if (++slot == DEPTH) slot = 0;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        x[j] = xn[j], x[j + 1] = xn[j + 1];
+        const float2 v = OT == F32 ? make_float2(on[j], on[j + 1]) : widen<OT>(hn[j / 2]);
+        t[j] = v.x, t[j + 1] = v.y;
+      }
+      if (more) fetch(row + gridDim.x);
     }
-    if (row + (int)gridDim.x < rows) fetch(row + gridDim.x);
     float f = 1.f;
     if (a.post_w) {
       float ss = 0.f;
@@ -197,9 +252,19 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? BLOCKS : 1) k_block_norms(
 // As many blocks as are resident at once go through the rows together.
 template <bool WIDE, int OT, int HT, int MAXT>
 static void launch(const Args& a, int rows, cudaStream_t st, const DrbDevice& dev) {
-  const int threads = ((a.d + V - 1) / V + 31) / 32 * 32;
-  const int fit = dev.sms * (MAXT == 128 ? BLOCKS * 128 / threads : 1);
-  drb_launch(k_block_norms<WIDE, OT, HT, MAXT>, dim3(rows < fit ? rows : fit), dim3(threads), 0, st, dev.pdl, a, rows);
+  const int threads = ((a.d + V - 1) / V + 31) / 32 * 32, smem = WIDE ? depth(MAXT) * threads * (64 + (OT == F32 ? 64 : 32)) : 0;
+  int fit = MAXT == 128 ? BLOCKS * 128 / threads : 1;
+  if (smem > 0 && fit > SMEM_MAX / smem) fit = SMEM_MAX / smem;
+  drb_launch(k_block_norms<WIDE, OT, HT, MAXT>, dim3(rows < dev.sms * fit ? rows : dev.sms * fit), dim3(threads), smem, st, dev.pdl, a, rows);
+}
+
+template <bool WIDE, int OT, int HT, int MAXT>
+static cudaError_t configure() {
+  if (WIDE) {
+    const cudaError_t e = cudaFuncSetAttribute(k_block_norms<WIDE, OT, HT, MAXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, depth(MAXT) * MAXT * 128);
+    if (e != cudaSuccess) return e;
+  }
+  return drb_carveout(k_block_norms<WIDE, OT, HT, MAXT>);
 }
 
 // The kernels for every pair of types, as one list for launches and set-up.
@@ -227,10 +292,10 @@ static cudaError_t configure_all() {
       const cudaError_t e = for_types(o, h, [](auto ot, auto ht) {
         constexpr int OT = decltype(ot)::value, HT = decltype(ht)::value;
         cudaError_t e;
-        if ((e = drb_carveout(k_block_norms<true, OT, HT, 128>)) != cudaSuccess) return e;
-        if ((e = drb_carveout(k_block_norms<true, OT, HT, 512>)) != cudaSuccess) return e;
-        if ((e = drb_carveout(k_block_norms<false, OT, HT, 128>)) != cudaSuccess) return e;
-        return drb_carveout(k_block_norms<false, OT, HT, 512>);
+        if ((e = configure<true, OT, HT, 128>()) != cudaSuccess) return e;
+        if ((e = configure<true, OT, HT, 512>()) != cudaSuccess) return e;
+        if ((e = configure<false, OT, HT, 128>()) != cudaSuccess) return e;
+        return configure<false, OT, HT, 512>();
       });
       if (e != cudaSuccess) return e;
     }
