@@ -5,6 +5,9 @@ region to the op before it for L2 prefetch (the last wraps to the first), and is
 into a graph that `step` replays — src/engine.rs:136-150 (`Op`), 674-708 (`record_step`),
 946-1042 (router + moe_decode per layer, x == res == y), 1047-1066 (`step`).
 
+Several requests decoding together, one row each: `MoeBatchDecoder` (drb_moe_few, one kernel a layer), `project_rows` (an int8 projection
+with each row's adapter) and `block_norms` (what lies between two blocks). No counterpart in the reference, which decodes at batch 1.
+
 Prefill: `MoePrefill` has two forms. `reference_calls=True` is src/engine.rs:544-604 call for call:
 cuBLAS router logits, dr_moe_topk, shared expert through dequant + cuBLAS, count, counts to the
 host, host exclusive scan, permute, grouped expert kernel, combine. The default is this library's
@@ -23,7 +26,7 @@ import numpy as np
 
 from . import ffi
 from .gpu import DevBuf, Graph, HostRow, Stream, check, launched
-from .model import MoeLayer
+from .model import Adapters, MoeLayer, Q8
 
 NULL = C.c_void_p(0)
 # src/engine.rs:18 has this switch off. Measured here as well: the warm-up runs in the router's single tail
@@ -354,3 +357,73 @@ class MoeStackDecoder:
         n = len(self.layers) * self.topk
         return (self.idx_trace.download(np.int32, n, self.st).reshape(-1, self.topk),
                 self.wts_trace.download(np.float32, n, self.st).reshape(-1, self.topk))
+
+
+class MoeBatchDecoder:
+    """Several requests decoding together over a stack of MoE layers: x[r] <- x[r] + moe_l(rmsnorm(x[r])) for each layer, one
+    kernel a layer (drb_moe_few). The batch has room for `streams` requests; rows that `set_live` switches off cost no expert and stay as they are,
+    also in a captured step. Results of a row do not depend on the others beyond the order of fp32 sums."""
+
+    def __init__(self, layers: list[MoeLayer], streams: int, topk: int = 8, eps: float = 1e-6, st: Stream | None = None) -> None:
+        self.l = ffi.lib()
+        self.st = st or Stream()
+        self.layers, self.streams, self.topk, self.eps = layers, streams, topk, eps
+        self.hidden, self.inter = layers[0].hidden, layers[0].inter
+        ws = self.l.drb_moe_few_workspace_bytes(streams, topk)
+        if ws < 0:
+            raise ValueError(f"drb_moe_few takes 1 to 16 rows and 1 to 8 experts a row, not {streams} and {topk}")
+        self.ws = DevBuf.zeros(ws, self.st)  # zeroed once; every call leaves it ready for the next
+        self.x = DevBuf(streams * self.hidden * 4)
+        self.row = HostRow(streams * self.hidden, self.st)
+        self.live = DevBuf.from_array(np.ones(streams, dtype=np.uint8), self.st)
+        self.weights = [ffi.MoeLayerPtrs(ly.router.ptr, ly.post_norm.ptr, ly.gate_up.q.ptr, ly.gate_up.sm.ptr, ly.down.q.ptr, ly.down.sm.ptr,
+                                         ly.shared_gate_up.q.ptr, ly.shared_gate_up.s.ptr, ly.shared_down.q.ptr, ly.shared_down.s.ptr) for ly in layers]
+        self.graph: Graph | None = None
+
+    def record_step(self) -> None:
+        for ly, w in zip(self.layers, self.weights):
+            launched(self.l.drb_moe_few(C.byref(w), self.x.at(0), self.x.at(0), self.live.at(0), self.streams, ly.experts, self.topk, self.hidden,
+                                        self.inter, self.eps, self.ws.at(0), self.st.raw), "moe_few")
+
+    def capture(self) -> None:
+        self.graph = Graph(self.st, self.record_step)
+
+    def set_live(self, live) -> None:
+        """Which rows are in use, one flag a row."""
+        flags = np.asarray(live, dtype=np.uint8)
+        assert flags.shape == (self.streams,)
+        self.live.upload(flags, self.st)
+
+    def set_x(self, x: np.ndarray) -> None:
+        assert x.shape == (self.streams, self.hidden)
+        self.row.put(self.x, x)
+
+    def step(self) -> np.ndarray:
+        """Replays the captured step (records it where none is captured) on the current rows and returns the new ones."""
+        if self.graph is not None:
+            self.graph.launch(self.st)
+        else:
+            self.record_step()
+        return self.row.get(self.x).reshape(self.streams, self.hidden)
+
+
+def project_rows(w: Q8, x, x_type: int, y, rows: int, st: Stream, adapters: Adapters | None = None, adapter_of=None, v=None, res=None) -> None:
+    """y [rows, n] f32 = x W^T (+ res) with each row's adapter beside it (drb_proj_q8_lora). x: 16-bit rows of x_type (1: bf16, 2: fp16);
+    adapter_of: int32 [rows], out of range = none; v: scratch f32 [rows, rank]. All are device buffers; y may be res."""
+    at = lambda b: b.at(0) if b is not None else NULL
+    q, s = w.rows(0)
+    if adapters is not None:
+        assert (adapters.n, adapters.k) == (w.n, w.k) and adapter_of is not None and v is not None
+    a = adapters
+    launched(ffi.lib().drb_proj_q8_lora(q, s, x.at(0), x_type, at(a and a.a), at(a and a.b), at(a and a.scale), at(adapter_of if a else None),
+                                        a.count if a else 0, a.rank if a else 0, at(res), y.at(0), at(v if a else None), rows, w.n, w.k, st.raw),
+             "proj_q8_lora")
+
+
+def block_norms(o, o_type: int, x, x_out, rows: int, d: int, st: Stream, post_w=None, gate=None, scale=None, alpha: float = 1.0, pre_w=None, h=None,
+                h_type: int = 1, eps: float = 1e-6) -> None:
+    """x_out = alpha x + sigmoid(gate) scale rmsnorm(o, post_w), h = rmsnorm(x_out, pre_w) (drb_block_norms); device buffers, types 0: f32, 1: bf16,
+    2: fp16; parts that are None are left out."""
+    at = lambda b: b.at(0) if b is not None else NULL
+    launched(ffi.lib().drb_block_norms(o.at(0), o_type, at(post_w), at(gate), at(scale), alpha, x.at(0), x_out.at(0), at(pre_w), at(h), h_type, rows, d, eps,
+                                       st.raw), "block_norms")

@@ -80,6 +80,27 @@ class Fp8Experts:
 
 
 @dataclass
+class Adapters:
+    """Low-rank adapters of one projection, resident together: a bf16 [count, rank, k], b bf16 [count, n, rank], scale f32 [count].
+    Adapters of a smaller rank are padded with zeros; rank is a multiple of 8."""
+
+    a: DevBuf
+    b: DevBuf
+    scale: DevBuf
+    count: int
+    rank: int
+    n: int
+    k: int
+
+    @classmethod
+    def upload(cls, a: np.ndarray, b: np.ndarray, scale: np.ndarray, st: Stream) -> "Adapters":
+        """a, b as uint16 bit patterns of bf16 numbers."""
+        count, rank, k = a.shape
+        assert b.shape[0] == count and b.shape[2] == rank and scale.shape == (count,) and a.dtype == b.dtype == np.uint16
+        return cls(DevBuf.from_array(a, st), DevBuf.from_array(b, st), DevBuf.from_array(scale.astype(np.float32), st), count, rank, b.shape[1], k)
+
+
+@dataclass
 class MoeLayer:
     router: DevBuf  # bf16 [E + 1, H]
     post_norm: DevBuf  # f32 [H]

@@ -64,7 +64,7 @@ def layer(e):
 
 
 @pytest.mark.parametrize("e,n,topk", [(16, 1, 8), (16, 2, 8), (16, 3, 1), (16, 16, 8), (33, 5, 3), (8, 9, 8), (1, 4, 1), (1, 16, 1), (64, 8, 6),
-                                      (64, 12, 2), (64, 7, 8), (64, 4, 8), (64, 13, 8)])
+                                      (64, 12, 2), (64, 7, 8), (64, 4, 8), (64, 13, 8), (8, 16, 8), (256, 1, 8), (256, 16, 8), (255, 3, 7)])
 def test_against_the_block(e, n, topk):
     st = Stream()
     few = Few(layer(e), n, topk, st)
@@ -90,4 +90,80 @@ def test_idle_rows_stay_as_they_were(n, live):
     assert_rows(y, ref, rows)
     assert (y[[i for i in range(n) if not live[i]]] == 7.0).all()
     assert np.array_equal(few.run(x, live), y)
+    assert device_error_word() == 0
+
+
+def test_equal_logits_go_to_the_lower_index():
+    host = dict(layer(64))
+    host["moe.router"] = np.zeros_like(host["moe.router"])
+    host["moe.router"][1::2] = synth.f32_to_bf16_bits(np.full((1, H), 2.0**-9, np.float32))  # the odd experts are equal, and so are the even ones
+    st = Stream()
+    few = Few(host, 3, 6, st)
+    x = np.abs(synth.make_x(9, 3, H))
+    x[1] = -x[1]  # the even experts' turn
+    y = few.run(x)
+    assert_rows(y, reference(host, x, 6), range(3))
+    assert device_error_word() == 0
+
+
+def test_rows_of_zeros_outliers_and_small_values():
+    st = Stream()
+    few = Few(layer(16), 6, 8, st)
+    x = synth.make_x(4, 6, H)
+    x[0] = 0
+    x[1, 100] = 3e4       # one input far above its neighbours
+    x[2] *= 1e-12         # eps rules the norm
+    x[3] *= 1e10
+    x[4, :64] = 0         # a group without a value
+    y = few.run(x)
+    ref = reference(layer(16), x, 8)
+    # the outlier sets the digits of its 63 neighbours: 2^-24 of it each, which carries the row's norm, through at most eight sums
+    assert np.array_equal(y[0], np.zeros(H, np.float32))
+    assert np.linalg.norm(y[1] - ref[1]) <= (REL + 8 * 64**0.5 * 2.0**-24) * np.linalg.norm(ref[1])
+    assert_rows(y, ref, (2, 3, 4, 5))
+    assert device_error_word() == 0
+
+
+@pytest.mark.parametrize("n", [3, 16])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_row_that_is_not_finite_touches_no_other(n, bad):
+    st = Stream()
+    few = Few(layer(64), n, 8, st)
+    x = synth.make_x(77, n, H)
+    x[1, 1234] = bad
+    live = [r != 1 for r in range(n)]
+    want = few.run(np.nan_to_num(x), live)
+    y = few.run(x)
+    assert np.isnan(y[1]).all()
+    ref = reference(layer(64), np.nan_to_num(x, posinf=0, neginf=0), 8)
+    assert_rows(y, ref, [r for r in range(n) if r != 1])
+    assert_rows(want, ref, [r for r in range(n) if r != 1])
+    assert device_error_word() == 0
+
+
+def test_one_workspace_serves_smaller_calls_and_other_layers():
+    st = Stream()
+    a = Few(layer(64), 16, 8, st)
+    x = synth.make_x(31, 16, H)
+    ya = a.run(x)
+    for n, topk in ((1, 1), (16, 8), (5, 3), (9, 8)):
+        y = a.run(x[:n], topk=topk)
+        assert_rows(y, reference(layer(64), x[:n], topk), range(n))
+    assert np.array_equal(a.run(x), ya)
+    b = Few(layer(16), 16, 8, st)
+    b.ws = a.ws
+    assert_rows(b.run(x), reference(layer(16), x, 8), range(16))
+    assert device_error_word() == 0
+
+
+def test_replays_are_the_same_bits():
+    st = Stream()
+    few = Few(layer(64), 7, 8, st)
+    x = synth.make_x(2, 7, H)
+    y = few.run(x)
+    dx, dy = DevBuf.from_array(x, st), DevBuf(7 * H * 4)
+    g = Graph(st, lambda: [launched(few.call(dx, dy), "moe_few") for _ in range(3)])
+    for _ in range(20):
+        g.launch(st)
+    assert np.array_equal(dy.download(np.float32, 7 * H, st).reshape(7, H), y)
     assert device_error_word() == 0
