@@ -254,7 +254,8 @@ template <bool WIDE, int OT, int HT, int MAXT>
 static void launch(const Args& a, int rows, cudaStream_t st, const DrbDevice& dev) {
   const int threads = ((a.d + V - 1) / V + 31) / 32 * 32, smem = WIDE ? depth(MAXT) * threads * (64 + (OT == F32 ? 64 : 32)) : 0;
   int fit = MAXT == 128 ? BLOCKS * 128 / threads : 1;
-  if (smem > 0 && fit > SMEM_MAX / smem) fit = SMEM_MAX / smem;
+  if constexpr (WIDE)
+    if (fit > SMEM_MAX / smem) fit = SMEM_MAX / smem;
   drb_launch(k_block_norms<WIDE, OT, HT, MAXT>, dim3(rows < dev.sms * fit ? rows : dev.sms * fit), dim3(threads), smem, st, dev.pdl, a, rows);
 }
 

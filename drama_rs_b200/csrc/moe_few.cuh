@@ -66,6 +66,7 @@ constexpr int TOKEN_BYTES = TOKEN_PLANES + MP * 16;
 constexpr int DEPTH = 4;
 constexpr int CTL_BYTES = 3072, PLANES_BYTES = TOK * TOKEN_PLANES, META_BYTES = TOK * MP * 16, RING_BYTES = CW * DEPTH * SLOT, RED_BYTES = CW * 16 * 8 * 4;
 constexpr size_t SMEM_BYTES = CTL_BYTES + PLANES_BYTES + META_BYTES + RING_BYTES + RED_BYTES;
+static_assert(8 * MAX_TOK <= SHARED_BLOCKS * CW, "a warp for every eighth of a token");
 static_assert(SMEM_BYTES <= 232448 && 2 * 3 * TOK * DPITCH <= PLANES_BYTES && 2 * TOK * DMP * 16 <= META_BYTES, "shared memory");
 static_assert((CTL_BYTES + PLANES_BYTES + META_BYTES) % 128 == 0 && SLOT % 128 == 0, "reads of the ring are told apart by their low bits");
 
@@ -159,7 +160,13 @@ struct Params {
   int n, e, topk;
   float eps;
   unsigned poll_limit;
+  // Divisions by what the host knows, by multiplication: of the grid; with one and with two halves of the shared expert, of the other
+  // blocks and of the blocks a group of four tokens (a dozen runtime divisions on a thread's way took 2 us)
+  unsigned long long by_grid, by_rest[2], by_per[2];
+  int per[2];
 };
+constexpr int RECIP_BITS = 40;  // x / d = x * ceil(2^40 / d) >> 40, exact while x * d < 2^40
+DRB_DEV unsigned times(unsigned x, unsigned long long recip) { return (unsigned)((x * recip) >> RECIP_BITS); }
 
 // One warp's share of a tile: 16 rows against the tokens of an entry. TG = 0: one or two tokens, four columns each (three digits); TG = 1: up
 // to eight, a column tile per digit. The sums: rows g and g + 8, or rows g (two), g + 8 (two) of tokens 2 t, 2 t + 1.
@@ -334,8 +341,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
   };
   // ---------------- logits: token group tg (four tokens), router rows [r0, r1); thread t holds inputs 4 t .. 4 t + 3. The rows come by copies
   // of each thread's own eight bytes into the planes, which are free so far; behind them the shared expert's weights are requested.
-  const int tgs = (n + 3) / 4, per = GN / tgs, tg = shared_block < 0 ? b / per : tgs;
-  const int r0 = tg < tgs ? E1 * (b % per) / per : 0, r1 = tg < tgs ? E1 * (b % per + 1) / per : 0;
+  const int tgs = (n + 3) >> 2, per = P.per[halves - 1], tg = shared_block < 0 ? (int)times(b, P.by_per[halves - 1]) : tgs;
+  const int part = b - tg * per;
+  const int r0 = tg < tgs ? times(E1 * part, P.by_per[halves - 1]) : 0, r1 = tg < tgs ? times(E1 * (part + 1), P.by_per[halves - 1]) : 0;
   {
     const unsigned char* src = static_cast<const unsigned char*>(P.w.router) + 8 * threadIdx.x;
     for (int r = r0; r < r1; ++r) cp8(smem_u32(planes + (r - r0) * 2 * H + 8 * threadIdx.x), src + (size_t)r * 2 * H);
@@ -358,6 +366,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
   if (threadIdx.x == 0) ctl.abort = 0;
   if (threadIdx.x < 20) (&ctl.arrived[0][0])[threadIdx.x] = 0;
   unsigned* done = P.ws->done[ep & 1];
+  // Digits: the shared expert's blocks, which have no logits to make, turn the tokens into them for all blocks, 256 inputs a warp
+  const int item = shared_block + warp * halves * SHARED_BLOCKS, itok = item >> 3;
+  if (shared_block >= 0 && item < 8 * n && ((live >> itok) & 1u)) {
+    unsigned char* dst = P.digits + (size_t)itok * TOKEN_BYTES;
+    const float4* xp = reinterpret_cast<const float4*>(P.x + (size_t)itok * H) + 64 * (item & 7) + lane;
+    const float4* np = reinterpret_cast<const float4*>(P.w.post_norm) + 64 * (item & 7) + lane;
+    const float4 x0 = __ldcg(xp), x1 = __ldcg(xp + 32), w0 = __ldcg(np), w1 = __ldcg(np + 32);
+    float4* mt = reinterpret_cast<float4*>(dst + TOKEN_PLANES) + 4 * (item & 7);
+    dst += 256 * (item & 7);
+    digits4(make_float4(x0.x * w0.x, x0.y * w0.y, x0.z * w0.z, x0.w * w0.w), dst, PITCH, mt, lane);
+    digits4(make_float4(x1.x * w1.x, x1.y * w1.y, x1.z * w1.z, x1.w * w1.w), dst + 128, PITCH, mt + 2, lane);
+    __syncwarp();
+    if (lane == 0) {
+      __threadfence();
+      atomicAdd(done + DIGITS, 1u);
+    }
+  }
+
   // Four sums over the warp (one for each token): lane l gets the one of token l >> 3
   auto sums4 = [&](float v0, float v1, float v2, float v3) {
     const bool hi = lane & 16, mid = lane & 8;
@@ -414,24 +440,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
         stack::ll_store(dst + 1, __float_as_uint(rr), tag);
         if (E & 1) stack::ll_store(dst + 2, 0u, tag);
       }
-    }
-  }
-
-  // Digits: warp w of block b turns 256 inputs of a token into them, for all blocks: eighth b + GN w of the n tokens
-  const int item = b + GN * warp, itok = item >> 3;
-  if (shared_block < 0 && item < 8 * n && ((live >> itok) & 1u)) {
-    unsigned char* dst = P.digits + (size_t)itok * TOKEN_BYTES;
-    const float4* xp = reinterpret_cast<const float4*>(P.x + (size_t)itok * H) + 64 * (item & 7) + lane;
-    const float4* np = reinterpret_cast<const float4*>(P.w.post_norm) + 64 * (item & 7) + lane;
-    const float4 x0 = __ldcg(xp), x1 = __ldcg(xp + 32), w0 = __ldcg(np), w1 = __ldcg(np + 32);
-    float4* mt = reinterpret_cast<float4*>(dst + TOKEN_PLANES) + 4 * (item & 7);
-    dst += 256 * (item & 7);
-    digits4(make_float4(x0.x * w0.x, x0.y * w0.y, x0.z * w0.z, x0.w * w0.w), dst, PITCH, mt, lane);
-    digits4(make_float4(x1.x * w1.x, x1.y * w1.y, x1.z * w1.z, x1.w * w1.w), dst + 128, PITCH, mt + 2, lane);
-    __syncwarp();
-    if (lane == 0) {
-      __threadfence();
-      atomicAdd(done + DIGITS, 1u);
     }
   }
 
@@ -605,21 +613,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
           if (ec > TOK) ctl.ent[h + 1] = (unsigned short)(threadIdx.x + 256);
           // gate/up: the shared expert's blocks have done SHARED_HEAD_START tiles already; down: its tiles come first, with twice the bytes
           const int lc = tile_cost(nlive), cs = lc + 4, ns = halves * SHARED_BLOCKS;
-          const int sum = GU_TILES * total, dsum = DN_TILES * (total + halves * cs), mine = min(sum, (sum + ns * SHARED_HEAD_START * lc) / G * GN);
+          const int sum = GU_TILES * total, dsum = DN_TILES * (total + halves * cs), mine = min(sum, (int)times(sum + ns * SHARED_HEAD_START * lc, P.by_grid) * GN);
           // lane q < 4: border q of this block (gate/up from, to; down from, to) on the scale of costs
           const int bb = b + (lane & 1);
           const bool late = !(lane & 2) && bb > GN;
-          const unsigned num = lane & 2 ? dsum * bb : late ? (sum - mine) * (bb - GN) : mine * bb, den = lane & 2 ? G : late ? ns : GN;
-          const int border = (int)(num / den) + (late ? mine : 0);
+          const unsigned num = lane & 2 ? dsum * bb : late ? (sum - mine) * (bb - GN) : mine * bb;
+          const int border = late ? mine + (int)(num / SHARED_BLOCKS >> (halves - 1)) : (int)times(num, lane & 2 ? P.by_grid : P.by_rest[halves - 1]);
 #pragma unroll 1
           for (int q = 0; q < 4; ++q) {
             const int at = __shfl_sync(0xffffffffu, border, q), scale = q < 2 ? GU_TILES : DN_TILES, heads = q < 2 ? 0 : halves, lead = heads * DN_TILES * cs;
             const int off = at - lead - scale * before;
-            const int round = q < 2 ? 4 : 1;  // a round of the four groups of warps
-            if (ec > 0 && off >= 0 && off < scale * c0) ctl.range[q] = (h + heads) * scale + (off + round * c0 - 1) / (round * c0) * round;
-            if (ec > TOK && off >= scale * c0 && off < scale * (c0 + c1))
-              ctl.range[q] = (h + heads + 1) * scale + (off - scale * c0 + round * c1 - 1) / (round * c1) * round;
-            if (threadIdx.x == 0 && at < lead) ctl.range[q] = (at + cs - 1) / cs;
+            // gate/up in whole rounds of the four groups of warps. Costs are 4 and 6: a third by multiplication (below 2^16)
+            const int round = q < 2 ? 4 : 1, lr = q < 2 ? 2 : 0;
+            const auto tiles = [&](int o, int c) { return (c == 4 ? (o + 4 * round - 1) >> (2 + lr) : ((o + 6 * round - 1) >> (1 + lr)) * 43691 >> 17) << lr; };
+            if (ec > 0 && off >= 0 && off < scale * c0) ctl.range[q] = (h + heads) * scale + tiles(off, c0);
+            if (ec > TOK && off >= scale * c0 && off < scale * (c0 + c1)) ctl.range[q] = (h + heads + 1) * scale + tiles(off - scale * c0, c1);
+            if (threadIdx.x == 0 && at < lead) ctl.range[q] = cs == 8 ? (at + 7) >> 3 : (at + 9) / 10;
             if (threadIdx.x == 0 && at >= lead + scale * total) ctl.range[q] = (nent + heads) * scale;
           }
         }
@@ -862,6 +871,13 @@ extern "C" int drb_moe_few(const drb_moe_layer* w, const float* x, float* y, con
   p.part = p.act + (size_t)n * (topk + 1) * few::I;
   p.digits = reinterpret_cast<unsigned char*>(p.part + (size_t)n * (topk + 1) * few::H);
   p.n = n, p.e = e, p.topk = topk, p.eps = eps, p.poll_limit = stack::POLL_LIMIT;
+  const auto recip = [](int d) { return ((1ull << few::RECIP_BITS) + d - 1) / d; };
+  p.by_grid = recip(dev.sms);
+  for (int halves = 1; halves <= 2; ++halves) {
+    const int rest = dev.sms - halves * few::SHARED_BLOCKS;
+    p.per[halves - 1] = rest / ((n + 3) / 4);
+    p.by_rest[halves - 1] = recip(rest), p.by_per[halves - 1] = recip(p.per[halves - 1]);
+  }
   void* args[] = {&p};
   const cudaError_t err = cudaLaunchCooperativeKernel((const void*)few::k_moe_few, dim3(dev.sms), dim3(few::THREADS), args, few::SMEM_BYTES, st);
   return err == cudaSuccess ? 0 : (int)err;
