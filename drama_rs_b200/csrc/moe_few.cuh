@@ -26,8 +26,6 @@
 
 #include <stddef.h>
 
-#include <type_traits>
-
 #include "gemv.cuh"
 #include "moe_decode.cuh"
 #include "stack_decode.cuh"
@@ -718,28 +716,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_moe_few(Params P) {
       if (!dn && tg) quad_sync(quad);
       Cols c;
       if (first < end) cols_set(c, tg, s, smem_u32(planes), pitch, smem_u32(meta), mp, lane);
-      auto steps = [&](auto tg_c, auto int8_c, float(&acc)[4]) {
-        constexpr bool INT8 = decltype(int8_c)::value;
-#pragma unroll
-        for (int sub = 0; sub < (INT8 ? 4 : 2); ++sub) {
-          cp_wait<DEPTH - 1>();
-          __syncwarp();
-          step<decltype(tg_c)::value, INT8>(acc, c, pitch, kg0 + (INT8 ? 2 : 4) * sub, slot + (INT8 ? at8 : at4), slot + (INT8 ? sc8 + 2 * sub : SUB + 16 * g));
-          __syncwarp();
-          issue(slot);
-          slot = slot + SLOT == ring_end ? ring : slot + SLOT;
-        }
-      };
-      using std::integral_constant;
+      const int nsub = int8 ? 4 : 2, kgs = int8 ? 2 : 4;
+      const uint32_t at = int8 ? at8 : at4, sc = int8 ? sc8 : SUB + 16 * g, scs = int8 ? 2 : 0;
 #pragma unroll 1
       for (; u < stop; u += nw) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        if (!int8) {
-          if (tg == 0) steps(integral_constant<int, 0>(), integral_constant<bool, false>(), acc);
-          else steps(integral_constant<int, 1>(), integral_constant<bool, false>(), acc);
-        } else {
-          if (tg == 0) steps(integral_constant<int, 0>(), integral_constant<bool, true>(), acc);
-          else steps(integral_constant<int, 1>(), integral_constant<bool, true>(), acc);
+        // One copy of the loop's requests for the four kinds of steps: the kernel runs through its code once or a few times, and every kilobyte of
+        // it comes from L2
+#pragma unroll 1
+        for (int sub = 0; sub < nsub; ++sub) {
+          cp_wait<DEPTH - 1>();
+          __syncwarp();
+          const int kg = kg0 + kgs * sub;
+          const uint32_t r = slot + at, q = slot + sc + scs * sub;
+          if (!int8) {
+            if (tg == 0) step<0, false>(acc, c, pitch, kg, r, q);
+            else step<1, false>(acc, c, pitch, kg, r, q);
+          } else {
+            if (tg == 0) step<0, true>(acc, c, pitch, kg, r, q);
+            else step<1, true>(acc, c, pitch, kg, r, q);
+          }
+          __syncwarp();
+          issue(slot);
+          slot = slot + SLOT == ring_end ? ring : slot + SLOT;
         }
         if (tg == 0) {  // the third digit's lanes join the first two's: rows g, g + 8 of token t >> 1
           acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 1);

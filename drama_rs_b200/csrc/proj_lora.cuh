@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   if (any)
     for (int i = cr * CW + warp; i < min(tw, t1 - t0) * 8 * NT; i += cs * CW) {
       const int a = __shfl_sync(0xffffffffu, ad, i % (8 * NT));
-      if (a >= 0 && 64 * half < p.rank) prefetch_line_l2(pair_row(t0 + i / (8 * NT), a) + 32 * half);
+      if (a >= 0 && 32 * half < p.rank) prefetch_line_l2(pair_row(t0 + i / (8 * NT), a) + 32 * half);
     }
   __syncthreads();
 
