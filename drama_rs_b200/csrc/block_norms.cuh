@@ -16,6 +16,7 @@
 namespace bn {
 
 constexpr int MAX_D = 8192;  // sixteen values a thread
+constexpr int MAX_ROWS = 1 << 30;  // a block looks a few thousand rows ahead: no row number passes 31 bits
 constexpr int BLOCKS = 5;    // of 128 threads a multiprocessor
 constexpr int depth(int maxt) { return maxt == 128 ? 4 : 3; }  // rows under way and in use
 constexpr int SMEM_MAX = 220 * 1024;  // of a multiprocessor, beside what the system takes of it
@@ -307,7 +308,7 @@ static cudaError_t configure_all() {
 
 extern "C" int drb_block_norms(const void* o, int o_type, const float* post_w, const float* gate, const float* scale, float alpha, const float* x,
                                float* x_out, const float* pre_w, void* h, int h_type, int rows, int d, float eps, cudaStream_t st) {
-  if (d < 1 || d > bn::MAX_D || rows < 0 || o_type < 0 || o_type > 2 || h_type < 0 || h_type > 2 || !o || !x || !x_out || (pre_w && !h)) return -1;
+  if (d < 1 || d > bn::MAX_D || rows < 0 || rows > bn::MAX_ROWS || o_type < 0 || o_type > 2 || h_type < 0 || h_type > 2 || !o || !x || !x_out || (pre_w && !h)) return -1;
   const auto off = [](const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; };
   // every value lies on a multiple of its own size
   if (off(o, o_type ? 2 : 4) || off(x, 4) || off(x_out, 4) || off(post_w, 4) || off(gate, 4) || off(scale, 4) || off(pre_w, 4) || (pre_w && off(h, h_type ? 2 : 4)))

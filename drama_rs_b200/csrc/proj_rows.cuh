@@ -58,6 +58,11 @@ DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
   }
 }
 
+// After a wait that ran out: the copies and multiplications that this block has asked for end within the millisecond.
+DRB_DEV void linger() {
+  for (int i = 0; i < 64; ++i) __nanosleep(16384);
+}
+
 template <bool F16>
 __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant__ Maps maps, pl::Args p, int nc, int tiles) {
   extern __shared__ unsigned char dyn_raw[];
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
     const uint32_t td = tmem + ((uint32_t)(32 * q) << 16);
     float acc[MAX_C];
     int wr = first * 128 + row;
-    auto scale = [&](int g) { return g < groups ? __ldg(p.s + (size_t)min(wr, p.n - 1) * groups + g) : __half(1.f); };
+    auto scale = [&](int g) { return __ldg(p.s + (size_t)min(wr, p.n - 1) * groups + min(g, groups - 1)); };
     __half nxt = mine > 0 ? scale(0) : __half();
     for (int c = 0, g = 0; c < total; ++c) {
       const __half h = nxt;
@@ -226,21 +231,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.accfree[c & 1]);
       };
+      if (g < groups) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (32 * j < nc) {
-          uint32_t d[32];
-          tmem_ld32(at + 32 * j, d);
-          if (32 * (j + 1) >= nc) drained();
+        for (int j = 0; j < 64; j += 32)
+          if (j < nc) {
+            uint32_t d[32];
+            tmem_ld32(at + j, d);
+            if (j + 32 >= nc) drained();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) acc[32 * j + e] = fmaf(f, __uint_as_float(d[e]), acc[32 * j + e]);
+            for (int e = 0; e < 32; ++e) acc[j + e] = fmaf(f, __uint_as_float(d[e]), acc[j + e]);
+          }
+        if (nc > 64) {
+          uint32_t d[16];
+          tmem_ld16(at + 64, d);
+          drained();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[64 + e] = fmaf(f, __uint_as_float(d[e]), acc[64 + e]);
         }
-      if (nc > 64) {
-        uint32_t d[16];
-        tmem_ld16(at + 64, d);
-        drained();
+      } else {
+        // an adapter's sums join its own rows alone: zeros of v against a NaN or an infinity of B are NaNs in every other row
+        const int ad = ctl.diff[g - groups];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[64 + e] = fmaf(f, __uint_as_float(d[e]), acc[64 + e]);
+        for (int j = 0; j < MAX_C; j += 16)
+          if (j < nc) {
+            const unsigned own = __ballot_sync(0xffffffffu, ctl.who[j + (lane & 15)] == ad);
+            uint32_t d[16];
+            tmem_ld16(at + j, d);
+            if (j + 16 >= nc) drained();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if ((own >> e) & 1u) acc[j + e] += __uint_as_float(d[e]);
+          }
       }
       if (++g == seq) {
         g = 0;
@@ -286,6 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
       __syncwarp();
       if (++g == seq) g = 0;
     }
+    if (spent) linger();
   } else {
     if (elect_one()) {
       if (p.rank == 0) pdl_wait();  // x
@@ -304,6 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
         while (wi < nw && wi < c / seq * groups + min(g, groups) + NRAW) load_w();
         if (++g == seq) g = 0;
       }
+      if (spent) linger();
     }
     __syncwarp();
   }
@@ -355,7 +378,7 @@ static cudaError_t configure_all() {
 extern "C" int drb_proj_q8_lora(const int8_t* w, const __half* s, const void* x, int x_type, const __nv_bfloat16* a, const __nv_bfloat16* b,
                                 const float* scale, const int* adapter_of, int adapters, int rank, const float* res, float* y, float* v, int rows, int n,
                                 int k, cudaStream_t st) {
-  if ((x_type != 1 && x_type != 2) || rows < 0 || n < 1 || k < 128 || k > pl::MAX_K || k % 128 || rank < 0 || rank > pl::MAX_RANK || rank % 8 || adapters < 0)
+  if ((x_type != 1 && x_type != 2) || rows < 0 || rows > 65535 * 64 || n < 1 || k < 128 || k > pl::MAX_K || k % 128 || rank < 0 || rank > pl::MAX_RANK || rank % 8 || adapters < 0)
     return -1;
   if (!w || !s || !x || !y || (rank > 0 && (!a || !b || !scale || !adapter_of || !v))) return -1;
   const auto off = [](const void* p, unsigned m) { return ((uintptr_t)p & (m - 1)) != 0; };
@@ -364,7 +387,6 @@ extern "C" int drb_proj_q8_lora(const int8_t* w, const __half* s, const void* x,
   const DrbDevice& dev = drb_device(st);
   if (!dev.ready) return -2;
   if (rows == 0) return 0;
-  if (rows > 65535 * 64) return -1;
   const pl::Args p = {w, s, x, a, b, scale, res, adapter_of, y, v, adapters, adapters > 0 ? rank : 0, rows, n, k};
   return x_type == 2 ? pr::launch_any<true>(p, dev, st) : pr::launch_any<false>(p, dev, st);
 }

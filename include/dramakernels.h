@@ -314,8 +314,9 @@ int drb_moe_few(const drb_moe_layer* w, const float* x, float* y, const uint8_t*
  * adapter_of: [rows], any order; res, y: f32 [rows, n], y may be res, res may be NULL; v: f32 scratch [rows, rank]. rank 0 (then a, b, scale,
  * adapter_of and v may be NULL) is the projection alone; adapters of a smaller rank are padded with zeros. Weights are not rounded: codes meet x
  * exactly, sums over the 128 inputs of a scale and everything behind them are f32. Two launches (one without adapters).
- * k a multiple of 128 up to 8192, rank a multiple of 8 up to 64, n >= 1, else -1; w, x, a, b and v 16-byte aligned, else -3. w and s are read
- * ahead of the launch before and must not be its work; everything else may be. */
+ * No row depends on another one, nor on another adapter than its own (a NaN there stays with its rows).
+ * k a multiple of 128 up to 8192, rank a multiple of 8 up to 64, n >= 1, rows <= 65535 * 64, else -1; w, x, a, b and v 16-byte aligned, else -3
+ * (also when the driver refuses a tensor map). w and s are read ahead of the launch before and must not be its work; everything else may be. */
 int drb_proj_q8_lora(const int8_t* w, const dr_half* s, const void* x, int x_type, const dr_bf16* a, const dr_bf16* b, const float* scale,
                      const int* adapter_of, int adapters, int rank, const float* res, float* y, float* v, int rows, int n, int k, dr_stream st);
 /* The norms between two blocks with the gate and the scaled residual between them, in one pass over [rows, d]:
@@ -323,7 +324,7 @@ int drb_proj_q8_lora(const int8_t* w, const dr_half* s, const void* x, int x_typ
  *   scale [d]: NULL = 1); h = rmsnorm(x_out, pre_w, eps) (pre_w NULL: no h is written and h may be NULL).
  * o of o_type and h of h_type (DRB_F32, DRB_BF16, DRB_F16; an fp16 h is clamped to +-65504, a NaN stays one), everything else f32. Sums in
  * fp32; a row's result does not depend on the number of rows. x_out may be x, and h may be o when their types are of one size.
- * 1 <= d <= 8192, else -1; any alignment of a value's own size (-3 otherwise), 16-byte aligned buffers and d % 4 == 0 are fastest.
+ * 1 <= d <= 8192, rows <= 2^30, else -1; any alignment of a value's own size (-3 otherwise), 16-byte aligned buffers and d % 4 == 0 are fastest.
  * All operands, weights too, may be the work of the launch before. */
 int drb_block_norms(const void* o, int o_type, const float* post_w, const float* gate, const float* scale, float alpha, const float* x,
                     float* x_out, const float* pre_w, void* h, int h_type, int rows, int d, float eps, dr_stream st);

@@ -67,3 +67,8 @@ def test_lora_refuses_shapes_types_and_missing_buffers(kw):
                                 dict(scale=A + 2), dict(who=A + 2)])
 def test_lora_refuses_misaligned_buffers(kw):
     assert lora(**kw) == -3
+
+
+def test_row_counts_have_a_limit():
+    assert norms(rows=2**30 + 1) == -1 and norms(rows=2**31 - 1, d=1) == -1
+    assert lora(rows=65535 * 64 + 1) == -1 and lora(rows=2**31 - 1) == -1

@@ -167,3 +167,33 @@ def test_replays_are_the_same_bits():
         g.launch(st)
     assert np.array_equal(dy.download(np.float32, 7 * H, st).reshape(7, H), y)
     assert device_error_word() == 0
+
+
+def test_two_calls_at_once():
+    """Two streams, a workspace each: every launch gets the whole device, one after the other."""
+    sts = [Stream(), Stream()]
+    few = [Few(layer(e), n, 8, st) for e, n, st in zip((64, 16), (3, 16), sts)]
+    xs = [synth.make_x(50 + f.n, f.n, H) for f in few]
+    want = [f.run(x) for f, x in zip(few, xs)]
+    dx = [DevBuf.from_array(x, st) for x, st in zip(xs, sts)]
+    dy = [DevBuf.zeros(x.nbytes, st) for x, st in zip(xs, sts)]
+    for st in sts:
+        st.sync()
+    for _ in range(30):
+        for f, x, y in zip(few, dx, dy):
+            launched(f.call(x, y), "moe_few")
+    for f, y, w, st in zip(few, dy, want, sts):
+        assert np.array_equal(y.download(np.float32, w.size, st).reshape(w.shape), w)
+    assert device_error_word() == 0
+
+
+def test_an_output_of_any_alignment():
+    st = Stream()
+    few = Few(layer(16), 5, 8, st)
+    x = synth.make_x(3, 5, H)
+    y = few.run(x)
+    dx, out = DevBuf.from_array(x, st), DevBuf.zeros(5 * H * 4 + 16, st)
+    w, live = few.w, None
+    launched(few.l.drb_moe_few(C.byref(w), dx.at(0), out.at(4), live, 5, 16, 8, H, I, EPS, few.ws.at(0), st.raw), "moe_few")
+    z = out.download(np.float32, 5 * H + 4, st)
+    assert np.array_equal(z[1 : 5 * H + 1].reshape(5, H), y) and z[0] == 0 and (z[5 * H + 1 :] == 0).all()

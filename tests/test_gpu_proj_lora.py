@@ -121,3 +121,52 @@ def test_a_row_of_nans_touches_no_other():
     t["x"][2, 17] = float("nan")
     z = run(t)
     assert torch.isnan(z[2]).all() and torch.equal(z[[0, 1, 3, 4, 5]], y[[0, 1, 3, 4, 5]])
+
+
+@pytest.mark.parametrize("rows", [6, 40, 70, 170])
+def test_a_broken_adapter_stays_with_its_own_rows(rows):
+    who = [r % 4 - 1 for r in range(rows)]
+    t = make(rows, rows, 300, 512, 3, 16, 1, who=who)
+    y = run(t)
+    t["b"][1, 7, 3] = float("nan")
+    t["b"][1, 9, 4] = float("inf")
+    t["a"][2, 5, 100] = float("nan")
+    z = run(t)
+    sound = [r for r in range(rows) if who[r] < 1]
+    assert torch.equal(z[sound], y[sound])
+    one = [r for r in range(rows) if who[r] == 1]
+    kept = [c for c in range(300) if c not in (7, 9)]
+    assert torch.isnan(z[one, 7]).all() and not torch.isfinite(z[one, 9]).any() and torch.equal(z[one][:, kept], y[one][:, kept])
+    assert torch.isnan(z[[r for r in range(rows) if who[r] == 2]]).all()
+
+
+@pytest.mark.parametrize("rows", [20, 90])
+def test_two_calls_at_once_and_a_replay(rows):
+    """Two streams with scratch of their own; then one of them captured, behind itself, and replayed."""
+    from drama_rs_b200.gpu import Graph
+
+    l, sts = ffi.lib(), [Stream(), Stream()]
+    ts = [make(40 + i, rows + 3 * i, 700, 1024, 3, 16, 1 + i) for i in range(2)]
+    ref = [run(t) for t in ts]
+    bufs, ys, vs = [], [], []
+    for t, st in zip(ts, sts):
+        bufs.append({name: up(t[name], st) for name in ("q", "s", "x", "a", "b", "scale", "who", "res")})
+        ys.append(DevBuf.zeros(t["dims"][0] * 700 * 4, st)), vs.append(DevBuf(t["dims"][0] * 16 * 4))
+
+    def call(i):
+        b, (n, *_) = bufs[i], ts[i]["dims"]
+        launched(l.drb_proj_q8_lora(*(b[m].at(0) for m in ("q", "s", "x")), 1 + i, *(b[m].at(0) for m in ("a", "b", "scale", "who")), 3, 16, b["res"].at(0),
+                                    ys[i].at(0), vs[i].at(0), n, 700, 1024, sts[i].raw), "proj_q8_lora")
+
+    def got(i):
+        n = ts[i]["dims"][0]
+        return torch.from_numpy(ys[i].download(np.float32, n * 700, sts[i]).reshape(n, 700))
+
+    for _ in range(20):
+        call(0), call(1)
+    assert torch.equal(got(0), ref[0]) and torch.equal(got(1), ref[1])
+    g = Graph(sts[0], lambda: (call(0), call(0)))
+    ys[0].zero(sts[0])
+    for _ in range(5):
+        g.launch(sts[0]), call(1)
+    assert torch.equal(got(0), ref[0]) and torch.equal(got(1), ref[1]) and device_error_word() == 0
