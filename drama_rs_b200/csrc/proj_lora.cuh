@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(256) k_shrink(Args p) {
   if (ad < 0) return;
   const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (size_t)row * p.k);
   const uint4* ap = reinterpret_cast<const uint4*>(p.a + ((size_t)ad * p.rank + j) * p.k);
+  const float scale = __ldcg(p.scale + ad);
   float acc[2] = {0.f, 0.f};
   for (int i0 = lane; i0 < p.k / 8; i0 += 8 * 32) {  // eight pieces of either at once
     uint4 xv[8], av[8];
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(256) k_shrink(Args p) {
     }
   }
   const float sum = warp_sum(acc[0] + acc[1]);
-  if (lane == 0) p.v[(size_t)row * p.rank + j] = sum * __ldcg(p.scale + ad);
+  if (lane == 0) p.v[(size_t)row * p.rank + j] = sum * scale;
 }
 
 template <bool F16>
@@ -117,10 +118,15 @@ DRB_DEV void split_f16(uint32_t h, uint32_t& hi, uint32_t& lo) {
   hi = *reinterpret_cast<const uint32_t*>(&a), lo = *reinterpret_cast<const uint32_t*>(&b);
 }
 
-// A block: eight ranks of sixteen rows, every adapter among them in turn; each of the eight warps an eighth of the inputs, in pieces of 32.
-// Rows are M, ranks are N; both operands straight from L2. fp16 rows meet the bf16 adapters as two bf16 terms.
+// A block: eight ranks of sixteen rows, every adapter among them in turn; each of the eight warps an eighth of the inputs, 64 at a time.
+// Rows are M, ranks are N; fp16 rows meet the bf16 adapters as two bf16 terms. x and A come by asynchronous copies of whole lines into
+// a ring of each warp's own (fragments straight from L2 are half lines, and beside the largest shared memory few lines of loads are under way at once:
+// 2 us for 64 inputs a warp). 256 threads of 64 registers and 52 KB are what a multiprocessor has left beside a block of k_proj_rows, which starts
+// while this kernel runs.
+constexpr int SH_STAGE = 24 * 128, SH_DEPTH = 2, SH_BYTES = 8 * SH_DEPTH * SH_STAGE;
 template <bool F16>
-__global__ void __launch_bounds__(256) k_shrink_rows(Args p) {
+__global__ void __launch_bounds__(256, 4) k_shrink_rows(Args p) {
+  extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ float part[8][16][8];
   const int row0 = (int)blockIdx.x * 16, j0 = (int)blockIdx.y * 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rows = min(16, p.rows - row0);
@@ -129,39 +135,56 @@ __global__ void __launch_bounds__(256) k_shrink_rows(Args p) {
   const int who = lane < rows ? adapter(p, row0 + lane) : -1;  // lane r: of row r
   const unsigned same = __match_any_sync(0xffffffffu, who);
   unsigned firsts = __ballot_sync(0xffffffffu, who >= 0 && __ffs(same) - 1 == lane);
-  const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(g, rows - 1)) * p.k + 8 * t;
-  const uint16_t* x1 = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min(g + 8, rows - 1)) * p.k + 8 * t;
-  const int steps = p.k / 32, c0 = steps * warp / 8, c1 = steps * (warp + 1) / 8;
+  const int groups = p.k / 64, c0 = groups * warp / 8, nc = groups * (warp + 1) / 8 - c0;
+  // Piece c (16 bytes) of row r lies where reads of two rows at once meet no bank twice. A lane copies piece lane % 8 of rows lane / 8, + 4, ...
+  const uint32_t ring = smem_u32(dyn) + warp * SH_DEPTH * SH_STAGE, put = (lane >> 3) * 128 + 16 * ((lane & 7) ^ (((lane >> 3) & 1) << 2));
+  const uint32_t get = g * 128 + 64 * (g & 1) + 16 * t;
+  const uint16_t* xr[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) xr[i] = static_cast<const uint16_t*>(p.x) + (size_t)(row0 + min((lane >> 3) + 4 * i, rows - 1)) * p.k + 64 * c0 + 8 * (lane & 7);
   for (; firsts; firsts &= firsts - 1u) {  // the different adapters
     const int r = __ffs(firsts) - 1, ad = __shfl_sync(0xffffffffu, who, r);
     const unsigned mine = __shfl_sync(0xffffffffu, same, r);
-    const uint16_t* ap = reinterpret_cast<const uint16_t*>(p.a) + ((size_t)ad * p.rank + j0 + g) * p.k + 8 * t;
-    float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
-    constexpr int FLY = F16 ? 4 : 8;  // pieces on the way at once
-    for (int c = c0; c < c1; c += FLY) {
-      uint4 u[FLY], v[FLY], b[FLY];
+    const float scale = __ldcg(p.scale + ad);
+    const uint16_t* ar = reinterpret_cast<const uint16_t*>(p.a) + ((size_t)ad * p.rank + j0 + (lane >> 3)) * p.k + 64 * c0 + 8 * (lane & 7);
+    auto issue = [&](int c) {
+      if (c < nc) {
+        const uint32_t dst = ring + (c & (SH_DEPTH - 1)) * SH_STAGE + put;
 #pragma unroll
-      for (int q = 0; q < FLY; ++q) {
-        const int at = 32 * min(c + q, c1 - 1);
-        u[q] = __ldcg(reinterpret_cast<const uint4*>(x0 + at)), v[q] = __ldcg(reinterpret_cast<const uint4*>(x1 + at));
-        b[q] = c + q < c1 ? __ldcg(reinterpret_cast<const uint4*>(ap + at)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i) few::cp16(dst + 512 * i, xr[i] + 64 * c);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) few::cp16(dst + 2048 + 512 * i, ar + (size_t)4 * i * p.k + 64 * c);
       }
+      few::cp_commit();
+    };
+    float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < FLY; ++q) {
+    for (int c = 0; c < SH_DEPTH; ++c) issue(c);
+#pragma unroll 1
+    for (int c = 0; c < nc; ++c) {
+      few::cp_wait<SH_DEPTH - 1>();
+      __syncwarp();
+      const uint32_t at = ring + (c & (SH_DEPTH - 1)) * SH_STAGE + get;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 u = few::lds<uint4>(at ^ (64 * h)), v = few::lds<uint4>((at ^ (64 * h)) + 1024), b = few::lds<uint4>((at ^ (64 * h)) + 2048);
         if constexpr (F16) {
           uint32_t uh[4], ul[4], vh[4], vl[4];
-          split_f16(u[q].x, uh[0], ul[0]), split_f16(u[q].y, uh[1], ul[1]), split_f16(u[q].z, uh[2], ul[2]), split_f16(u[q].w, uh[3], ul[3]);
-          split_f16(v[q].x, vh[0], vl[0]), split_f16(v[q].y, vh[1], vl[1]), split_f16(v[q].z, vh[2], vl[2]), split_f16(v[q].w, vh[3], vl[3]);
-          mma16<false>(d, uh[0], vh[0], uh[1], vh[1], b[q].x, b[q].y);
-          mma16<false>(e, uh[2], vh[2], uh[3], vh[3], b[q].z, b[q].w);
-          mma16<false>(d, ul[0], vl[0], ul[1], vl[1], b[q].x, b[q].y);
-          mma16<false>(e, ul[2], vl[2], ul[3], vl[3], b[q].z, b[q].w);
+          split_f16(u.x, uh[0], ul[0]), split_f16(u.y, uh[1], ul[1]), split_f16(u.z, uh[2], ul[2]), split_f16(u.w, uh[3], ul[3]);
+          split_f16(v.x, vh[0], vl[0]), split_f16(v.y, vh[1], vl[1]), split_f16(v.z, vh[2], vl[2]), split_f16(v.w, vh[3], vl[3]);
+          mma16<false>(d, uh[0], vh[0], uh[1], vh[1], b.x, b.y);
+          mma16<false>(e, uh[2], vh[2], uh[3], vh[3], b.z, b.w);
+          mma16<false>(d, ul[0], vl[0], ul[1], vl[1], b.x, b.y);
+          mma16<false>(e, ul[2], vl[2], ul[3], vl[3], b.z, b.w);
         } else {
-          mma16<false>(d, u[q].x, v[q].x, u[q].y, v[q].y, b[q].x, b[q].y);
-          mma16<false>(e, u[q].z, v[q].z, u[q].w, v[q].w, b[q].z, b[q].w);
+          mma16<false>(d, u.x, v.x, u.y, v.y, b.x, b.y);
+          mma16<false>(e, u.z, v.z, u.w, v.w, b.z, b.w);
         }
       }
+      __syncwarp();
+      issue(c + SH_DEPTH);
     }
+    few::cp_wait<0>();
     *reinterpret_cast<float2*>(&part[warp][g][2 * t]) = make_float2(d[0] + e[0], d[1] + e[1]);
     *reinterpret_cast<float2*>(&part[warp][g + 8][2 * t]) = make_float2(d[2] + e[2], d[3] + e[3]);
     __syncthreads();
@@ -170,7 +193,7 @@ __global__ void __launch_bounds__(256) k_shrink_rows(Args p) {
       float s = 0.f;
 #pragma unroll
       for (int q = 0; q < 8; ++q) s += part[q][m][j];
-      p.v[(size_t)(row0 + m) * p.rank + j0 + j] = s * __ldcg(p.scale + ad);
+      p.v[(size_t)(row0 + m) * p.rank + j0 + j] = s * scale;
     }
     __syncthreads();
   }
@@ -493,7 +516,7 @@ static int launch_few(const Args& p, const DrbDevice& dev, cudaStream_t st) {
 
 template <bool F16>
 static void launch_shrink(const Args& p, const DrbDevice& dev, cudaStream_t st) {
-  if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
+  if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
   else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
 }
 
@@ -509,6 +532,7 @@ static cudaError_t configure_type() {
   if ((e = configure<F16, 2>()) != cudaSuccess) return e;
   if ((e = configure<F16, 3>()) != cudaSuccess) return e;
   if ((e = configure<F16, 4>()) != cudaSuccess) return e;
+  if ((e = cudaFuncSetAttribute(k_shrink_rows<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SH_BYTES)) != cudaSuccess) return e;
   if ((e = drb_carveout(k_shrink_rows<F16>)) != cudaSuccess) return e;
   return drb_carveout(k_shrink<F16>);
 }

@@ -21,7 +21,11 @@ namespace pr {
 
 using namespace tc;
 
-constexpr int CONV = 8, SET = 4, SETS = CONV / SET, EPI = 4, MMA_WARP = CONV + EPI, LOAD_WARP = MMA_WARP + 1, THREADS = (LOAD_WARP + 1) * 32;
+constexpr int CONV = 8, SET = 4, SETS = CONV / SET, EPI = 4, MMA_WARP = CONV + EPI, LOAD_WARP = MMA_WARP + 1, WHO_WARP = LOAD_WARP + 1, THREADS = 512;
+// Registers a thread: what the launch gets, and after the roles have parted (setmaxnreg works on groups of four warps; the sixteenth only gives
+// its own). The shares are no more than the launch's.
+constexpr int LAUNCH_REGS = 96, CONV_REGS = 88, EPI_REGS = 144, REST_REGS = 64;
+static_assert(8 * CONV_REGS + 4 * EPI_REGS + 4 * REST_REGS <= THREADS / 32 * LAUNCH_REGS && CONV == 8 && EPI == 4, "registers");
 constexpr int NRAW = 4, NA = 3;            // raw stages of 16 KB; stages of A (64 columns of tensor memory) with a tile of x
 constexpr int MAX_C = 80;                  // rows of x a tile: their sums are an epilogue thread's registers
 constexpr int RAW_BYTES = 128 * 128;
@@ -33,7 +37,7 @@ struct Ctl {
   uint64_t full[NA], done[NA];             // a stage is complete (convert warps, and the tile of x) / its multiplications have completed
   uint64_t accfull[2], accfree[2];         // an accumulator is complete / has been drained (one arrival per epilogue warp)
   uint32_t tmem;
-  unsigned firsts[3];
+  int ndiff;
   __align__(16) int who[96];            // adapters of the tile's rows, -1: none
   int diff[MAX_C];                         // the different ones among them
 };
@@ -64,7 +68,7 @@ DRB_DEV void linger() {
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant__ Maps maps, pl::Args p, int nc, int tiles) {
+__global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Maps maps, pl::Args p, int nc, int tiles) {
   extern __shared__ unsigned char dyn_raw[];
   unsigned char* dyn = dyn_raw + (-smem_u32(dyn_raw) & 1023u);
   Ctl& ctl = *reinterpret_cast<Ctl*>(dyn);
@@ -99,34 +103,42 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
   }
   if (warp == MMA_WARP) tmem_alloc(&ctl.tmem, TMEM_COLS);
   pdl_launch_dependents();
-  // The tile's adapters and the different ones among them. With adapters x and adapter_of are older than the launch before (see proj_lora.cuh).
-  const int a = p.rank > 0 && (int)threadIdx.x < cols ? pl::adapter(p, row0 + threadIdx.x) : -1;
-  if (threadIdx.x < 96) ctl.who[threadIdx.x] = a;
+  // The tile's adapters, a lane three of them, and the different ones among them. With adapters x and adapter_of are older than the launch before
+  // (see proj_lora.cuh).
+  if (warp == WHO_WARP && p.rank > 0) {
+    int a[3], n = 0;
+    bool is_first[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) a[i] = 32 * i + lane < cols ? pl::adapter(p, row0 + 32 * i + lane) : -1;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      ctl.who[32 * i + lane] = a[i];
+      const unsigned same = __match_any_sync(0xffffffffu, a[i]);
+      is_first[i] = a[i] >= 0 && __ffs(same) - 1 == lane;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const unsigned firsts = __ballot_sync(0xffffffffu, is_first[i]);
+      if (is_first[i]) ctl.diff[n + __popc(firsts & ((1u << lane) - 1u))] = a[i];
+      n += __popc(firsts);
+      for (unsigned m = firsts; m; m &= m - 1u) {
+        const int ad = __shfl_sync(0xffffffffu, a[i], __ffs(m) - 1);
+#pragma unroll
+        for (int k = i + 1; k < 3; ++k) is_first[k] = is_first[k] && a[k] != ad;
+      }
+    }
+    if (lane == 0) ctl.ndiff = n;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl.tmem;
-  int ndiff = 0;
-  if (p.rank > 0) {
-    if (threadIdx.x < 96) {
-      bool is_first = a >= 0;
-#pragma unroll 8
-      for (int j = 0; j < (int)threadIdx.x; j += 4) {
-        const int4 w = *reinterpret_cast<const int4*>(&ctl.who[j]);
-        const int left = (int)threadIdx.x - j;
-        is_first = is_first && w.x != a && !(left > 1 && w.y == a) && !(left > 2 && w.z == a) && !(left > 3 && w.w == a);
-      }
-      const unsigned f = __ballot_sync(0xffffffffu, is_first);
-      if (lane == 0) ctl.firsts[warp] = f;
-    }
-    __syncthreads();
-    const unsigned f0 = ctl.firsts[0], f1 = ctl.firsts[1], f2 = ctl.firsts[2];
-    ndiff = __popc(f0) + __popc(f1) + __popc(f2);
-    if (threadIdx.x < 96 && (ctl.firsts[warp] >> lane) & 1u)
-      ctl.diff[(warp > 0 ? __popc(f0) : 0) + (warp > 1 ? __popc(f1) : 0) + __popc(ctl.firsts[warp] & ((1u << lane) - 1u))] = a;
-    __syncthreads();
-  }
+  const int ndiff = p.rank > 0 ? ctl.ndiff : 0;
   const int seq = groups + ndiff, total = mine * seq;  // stretches of inputs: a tile's 128s, then its adapters
+
+  if (warp < CONV) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONV_REGS));
+  else if (warp < MMA_WARP) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REST_REGS));
 
   if (warp < CONV) {
     // ---------------- convert: two sets of four warps take turns at the stretches; a thread has one row of the tile
@@ -170,21 +182,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
           const uint4 b = 8 * j < p.rank ? __ldcg(bp + j) : make_uint4(0u, 0u, 0u, 0u);
           o[4 * j] = b.x, o[4 * j + 1] = b.y, o[4 * j + 2] = b.z, o[4 * j + 3] = b.w;
         }
-        if (use > 0) mbar_wait_ring<DRB_ERR_TMEM>(smem_u32(&ctl.done[s]), (use - 1) & 1, spent);
-        tc_fence_after();
-        tmem_st32(ta + 64 * s, o);
         if (!awaited) pdl_wait(), awaited = true;
-        unsigned char* xs = xst + s * xstage;
         // four ranks of a row a thread, five rows at once: thread i takes ranks 4 (i % 16) .. of rows i / 16, i / 16 + 8, ...
         const int k4 = threadIdx.x & 15;
-        for (int r0 = (threadIdx.x & (SET * 32 - 1)) >> 4; r0 < nc; r0 += 40) {
-          float4 f[5];
+        float4 f[5];
+        auto load_v = [&](int r0) {
 #pragma unroll
           for (int i = 0; i < 5; ++i) {
             const int r = r0 + 8 * i;
             f[i] = r < nc && ctl.who[r] == ad && 4 * k4 < p.rank ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + k4)
                                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
           }
+        };
+        int r0 = (threadIdx.x & (SET * 32 - 1)) >> 4;
+        load_v(r0);
+        if (use > 0) mbar_wait_ring<DRB_ERR_TMEM>(smem_u32(&ctl.done[s]), (use - 1) & 1, spent);
+        tc_fence_after();
+        tmem_st32(ta + 64 * s, o);
+        unsigned char* xs = xst + s * xstage;
+        for (;;) {
 #pragma unroll
           for (int i = 0; i < 5; ++i) {
             const int r = r0 + 8 * i;
@@ -194,6 +210,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
 #pragma unroll
             for (int l = 0; l < 3; ++l) *reinterpret_cast<uint2*>(xs + l * box + swz_off(r, k4 >> 1) + 8 * (k4 & 1)) = make_uint2(b0[l], b1[l]);
           }
+          if ((r0 += 40) >= nc) break;
+          load_v(r0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the multiplications read v through the asynchronous proxy
       }
@@ -308,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
       if (++g == seq) g = 0;
     }
     if (spent) linger();
-  } else {
+  } else if (warp == LOAD_WARP) {
     if (elect_one()) {
       if (p.rank == 0) pdl_wait();  // x
       for (int c = 0, g = 0; c < total; ++c) {
@@ -329,6 +347,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_proj_rows(const __grid_constant_
       if (spent) linger();
     }
     __syncwarp();
+  } else if (warp == WHO_WARP) {  // the adapters' rows of B for the first tile come to L2 meanwhile
+    for (int i = 0; i < ndiff; ++i)
+      for (int r = lane; r < 128; r += 32) prefetch_line_l2(p.b + ((size_t)ctl.diff[i] * p.n + min(first * 128 + r, p.n - 1)) * p.rank);
   }
   tc_fence_before();
   __syncthreads();
@@ -369,6 +390,9 @@ static cudaError_t configure_all() {
   cudaError_t e;
   if ((e = cudaFuncSetAttribute(k_proj_rows<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(MAX_C))) != cudaSuccess) return e;
   if ((e = cudaFuncSetAttribute(k_proj_rows<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(MAX_C))) != cudaSuccess) return e;
+  cudaFuncAttributes a, b;  // with fewer registers at the launch than the shares add up to the warps would wait for the rest
+  if ((e = cudaFuncGetAttributes(&a, k_proj_rows<true>)) != cudaSuccess || (e = cudaFuncGetAttributes(&b, k_proj_rows<false>)) != cudaSuccess) return e;
+  if (a.numRegs < LAUNCH_REGS || b.numRegs < LAUNCH_REGS) return cudaErrorInvalidConfiguration;
   if ((e = drb_carveout(k_proj_rows<true>)) != cudaSuccess) return e;
   return drb_carveout(k_proj_rows<false>);
 }
