@@ -46,27 +46,46 @@ DRB_DEV int adapter(const Args& p, int row) {  // -1: none
 }
 
 // ---- v = scale A x ------------------------------------------------------------------------------------------------------
-// A block: eight ranks of one row, a warp each.
+// A block: eight ranks of one row, a warp each. Up to SK inputs of x and of the eight rows of A come by asynchronous copies at once: plain loads
+// are few lines at a time beside the largest shared memory, and their registers kept blocks of k_proj off the multiprocessor.
+constexpr int SK = 4096;
+static int shrink_bytes(int k) { return 9 * 2 * (k < SK ? k : SK); }
 template <bool F16>
-__global__ void __launch_bounds__(256) k_shrink(Args p) {
-  const int row = (int)blockIdx.x, j = (int)blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(256, 6) k_shrink(Args p) {
+  extern __shared__ __align__(128) unsigned char dyn[];
+  const int row = (int)blockIdx.x, warp = threadIdx.x >> 5, j = (int)blockIdx.y * 8 + warp, lane = threadIdx.x & 31;
+  const int most = min(p.k, SK);
+  const uint32_t xs = smem_u32(dyn), as = xs + 2 * most * (1 + warp);
+  const uint16_t* xp = static_cast<const uint16_t*>(p.x) + (size_t)row * p.k;
   pdl_wait();
   pdl_launch_dependents();  // behind the wait: see above
+  auto load_x = [&](int k0) {
+    for (int i = threadIdx.x; i < min(SK, p.k - k0) / 8; i += 256) few::cp16(xs + 16 * i, xp + k0 + 8 * i);
+  };
+  load_x(0);
   const int ad = adapter(p, row);
-  if (ad < 0) return;
-  const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (size_t)row * p.k);
-  const uint4* ap = reinterpret_cast<const uint4*>(p.a + ((size_t)ad * p.rank + j) * p.k);
+  if (ad < 0) {
+    few::cp_commit();
+    few::cp_wait<0>();
+    return;
+  }
+  const __nv_bfloat16* ap = p.a + ((size_t)ad * p.rank + j) * p.k;
   const float scale = __ldcg(p.scale + ad);
   float acc[2] = {0.f, 0.f};
-  for (int i0 = lane; i0 < p.k / 8; i0 += 8 * 32) {  // eight pieces of either at once
-    uint4 xv[8], av[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (i0 + 32 * q < p.k / 8) xv[q] = __ldcg(xp + i0 + 32 * q), av[q] = __ldcg(ap + i0 + 32 * q);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      if (i0 + 32 * q >= p.k / 8) break;
-      const uint32_t xw[4] = {xv[q].x, xv[q].y, xv[q].z, xv[q].w}, aw[4] = {av[q].x, av[q].y, av[q].z, av[q].w};
+  for (int k0 = 0; k0 < p.k; k0 += SK) {
+    if (k0 > 0) {
+      __syncthreads();
+      load_x(k0);
+    }
+    const int n = min(SK, p.k - k0) / 8;
+    for (int i = lane; i < n; i += 32) few::cp16(as + 16 * i, ap + k0 + 8 * i);
+    few::cp_commit();
+    few::cp_wait<0>();
+    __syncthreads();
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) {
+      const uint4 xv = few::lds<uint4>(xs + 16 * i), av = few::lds<uint4>(as + 16 * i);
+      const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, aw[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         acc[0] = fmaf(widen16(xw[e] & 0xffffu, F16), widen16(aw[e] & 0xffffu, false), acc[0]);
@@ -517,7 +536,7 @@ static int launch_few(const Args& p, const DrbDevice& dev, cudaStream_t st) {
 template <bool F16>
 static void launch_shrink(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
-  else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), 0, st, dev.pdl, p);
+  else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), shrink_bytes(p.k), st, dev.pdl, p);
 }
 
 template <bool F16, int NT>
@@ -534,6 +553,7 @@ static cudaError_t configure_type() {
   if ((e = configure<F16, 4>()) != cudaSuccess) return e;
   if ((e = cudaFuncSetAttribute(k_shrink_rows<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SH_BYTES)) != cudaSuccess) return e;
   if ((e = drb_carveout(k_shrink_rows<F16>)) != cudaSuccess) return e;
+  if ((e = cudaFuncSetAttribute(k_shrink<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, shrink_bytes(SK))) != cudaSuccess) return e;
   return drb_carveout(k_shrink<F16>);
 }
 static cudaError_t configure_all() {
