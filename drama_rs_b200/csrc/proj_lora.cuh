@@ -25,7 +25,7 @@ constexpr int CW = 8, THREADS = CW * 32;
 constexpr int SUB = 2048;                  // a step of a warp: 16 weight rows x 128 inputs
 constexpr int DEPTH = 3;
 constexpr int PP = 20;                     // floats between the columns of a tile of sums: writes of a warp meet no bank twice
-constexpr size_t SMEM_MAX = 232448, SMEM_TWO = 112 * 1024;  // up to the second, two blocks share a multiprocessor
+constexpr size_t SMEM_MAX = 232448, SMEM_TWO = 113 * 1024;  // up to the second, two blocks share a multiprocessor
 constexpr int TILE_ROWS = 64;              // up to so many rows: k_shrink and k_proj, beyond: k_shrink_rows and k_proj_rows
 
 struct Args {
@@ -137,6 +137,17 @@ DRB_DEV void split_f16(uint32_t h, uint32_t& hi, uint32_t& lo) {
   hi = *reinterpret_cast<const uint32_t*>(&a), lo = *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// Four fp32 numbers as pairs of bf16 numbers in three terms (eight bits each, the third rounded).
+DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
+  float4 r = v;
+#pragma unroll
+  for (int l = 0; l < 3; ++l) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(r.x, r.y), c = __floats2bfloat162_rn(r.z, r.w);
+    b0[l] = *reinterpret_cast<const uint32_t*>(&a), b1[l] = *reinterpret_cast<const uint32_t*>(&c);
+    r = make_float4(r.x - __low2float(a), r.y - __high2float(a), r.z - __low2float(c), r.w - __high2float(c));
+  }
+}
+
 // A block: eight ranks of sixteen rows, every adapter among them in turn; each of the eight warps an eighth of the inputs, 64 at a time.
 // Rows are M, ranks are N; fp16 rows meet the bf16 adapters as two bf16 terms. x and A come by asynchronous copies of whole lines into
 // a ring of each warp's own (fragments straight from L2 are half lines, and beside the largest shared memory few lines of loads are under way at once:
@@ -234,11 +245,15 @@ DRB_DEV float4 ld_peer(uint32_t addr, unsigned rank) {
   return v;
 }
 
+// v of a row: three terms (see split3) of 64 ranks, pieces of eight ranks where reads of two terms at once meet no bank twice
+constexpr int V_BYTES = 3 * MAX_RANK * 2;
+DRB_DEV uint32_t v_at(int term, int piece) { return 128 * term + 16 * (piece ^ ((term & 1) << 2)); }
+
 // NT column tiles (8 rows of x each) a pass; a slice of K inputs.
 template <int NT>
 struct Shape {
   static constexpr size_t SUMS = (size_t)CW * 8 * NT * PP * 4, RING = (size_t)CW * DEPTH * SUB;
-  static constexpr size_t VS = (size_t)8 * NT * (MAX_RANK + 4) * 4;  // v of the pass
+  static constexpr size_t VS = (size_t)8 * NT * V_BYTES;  // v of the pass
   static constexpr size_t bytes(int slice) { return 256 + (size_t)8 * NT * (2 * slice + 16) + SUMS + RING + VS; }
 };
 static_assert(Shape<4>::bytes(MAX_K / 8) <= SMEM_MAX, "eight blocks hold the longest row");
@@ -256,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   int* who = reinterpret_cast<int*>(dyn);  // adapters of the pass's rows
   unsigned char* xs = dyn + 256;
   float* sums = reinterpret_cast<float*>(xs + (size_t)8 * NT * sp.pitch);
-  float* vs = sums + Shape<NT>::SUMS / 4;
+  unsigned char* vs = reinterpret_cast<unsigned char*>(sums) + Shape<NT>::SUMS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(vs) + Shape<NT>::VS + warp * DEPTH * SUB;
   const int lcs = sp.lcs, lkw = sp.lkw, cs = 1 << lcs, kw = 1 << lkw, pitch = sp.pitch;
@@ -331,8 +346,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   }
   const bool any = __ballot_sync(0xffffffffu, ad >= 0) != 0u;  // the same in every warp
   if (warp == 0) who[lane] = ad;
-  // The adapters' second half: a warp takes the sixteen weight rows of a tile for a row of x, two lanes a weight row; the pairs of a batch are dealt out
-  // over the cluster and its warps. The rows of B for the first batch come to L2 meanwhile.
+  // The adapters' second half: a warp takes the sixteen weight rows of a tile for a row of x, whose v is the other operand, a term a column; the pairs
+  // of a batch are dealt out over the cluster and its warps. The rows of B for the first batch come to L2 meanwhile.
   const int lr = lane >> 1, half = lane & 1;
   auto pair_row = [&](int tile, int a) { return p.b + ((size_t)a * p.n + min(16 * tile + lr, p.n - 1)) * p.rank; };
   if (any)
@@ -396,9 +411,12 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
       if (any) {
         for (int i = threadIdx.x; i < 8 * NT * (MAX_RANK / 4); i += THREADS) {
           const int r = i / (MAX_RANK / 4), q = i % (MAX_RANK / 4);
-          if (4 * q >= p.rank) continue;
-          *reinterpret_cast<float4*>(vs + r * (MAX_RANK + 4) + 4 * q) =
-              r < cols && who[r] >= 0 ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 f = r < cols && who[r] >= 0 && 4 * q < p.rank ? __ldcg(reinterpret_cast<const float4*>(p.v + (size_t)(row0 + r) * p.rank) + q)
+                                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+          uint32_t b0[3], b1[3];
+          split3(f, b0, b1);
+#pragma unroll
+          for (int l = 0; l < 3; ++l) *reinterpret_cast<uint2*>(vs + r * V_BYTES + v_at(l, q >> 1) + 8 * (q & 1)) = make_uint2(b0[l], b1[l]);
         }
         __syncthreads();
       }
@@ -414,36 +432,40 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
     const int nt = min(tw, t1 - t0 - bt * tw);
     if (any) {
       __syncthreads();
-      constexpr int PAIRS = 8;  // on the way at once
+      constexpr int PAIRS = NT == 1 ? 2 : 4;  // on the way at once: of few pairs a warp has one or two, and every one more is code to fetch
       for (int i0 = cr * CW + warp; i0 < nt * 8 * NT; i0 += PAIRS * cs * CW) {
-        float a[PAIRS];
-        const uint4* bp[PAIRS];
-        int r[PAIRS];
+        float d[PAIRS][4];
+        const __nv_bfloat16* bp[PAIRS];  // this lane's row g; row g + 8 lies `down` numbers on
+        int r[PAIRS], down[PAIRS];
 #pragma unroll
         for (int e = 0; e < PAIRS; ++e) {
-          const int i = i0 + e * cs * CW;
-          r[e] = i % (8 * NT), a[e] = 0.f;
-          bp[e] = who[r[e]] < 0 || i >= nt * 8 * NT ? nullptr : reinterpret_cast<const uint4*>(pair_row(t0 + bt * tw + i / (8 * NT), who[r[e]])) + half;
+          const int i = i0 + e * cs * CW, o = 16 * (t0 + bt * tw + i / (8 * NT)) + g;
+          r[e] = i % (8 * NT), d[e][0] = d[e][1] = d[e][2] = d[e][3] = 0.f;
+          bp[e] = who[r[e]] < 0 || i >= nt * 8 * NT ? nullptr : p.b + ((size_t)who[r[e]] * p.n + min(o, p.n - 1)) * p.rank + 8 * t;
+          down[e] = (min(o + 8, p.n - 1) - min(o, p.n - 1)) * p.rank;
         }
-        for (int q = half; q < p.rank / 8; q += 2) {
-          uint4 bw[PAIRS];
-#pragma unroll
-          for (int e = 0; e < PAIRS; ++e) bw[e] = bp[e] ? __ldcg(bp[e] + (q - half)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int q = 0; q < p.rank; q += 32) {
+          uint4 u[PAIRS], v[PAIRS];
 #pragma unroll
           for (int e = 0; e < PAIRS; ++e) {
-            const float4* vp = reinterpret_cast<const float4*>(vs + r[e] * (MAX_RANK + 4) + 8 * q);
-            const float4 v0 = vp[0], v1 = vp[1];
-            a[e] = fmaf(widen16(bw[e].x & 0xffffu, false), v0.x, a[e]), a[e] = fmaf(widen16(bw[e].x >> 16, false), v0.y, a[e]);
-            a[e] = fmaf(widen16(bw[e].y & 0xffffu, false), v0.z, a[e]), a[e] = fmaf(widen16(bw[e].y >> 16, false), v0.w, a[e]);
-            a[e] = fmaf(widen16(bw[e].z & 0xffffu, false), v1.x, a[e]), a[e] = fmaf(widen16(bw[e].z >> 16, false), v1.y, a[e]);
-            a[e] = fmaf(widen16(bw[e].w & 0xffffu, false), v1.z, a[e]), a[e] = fmaf(widen16(bw[e].w >> 16, false), v1.w, a[e]);
+            u[e] = v[e] = make_uint4(0u, 0u, 0u, 0u);
+            if (bp[e] && q + 8 * t < p.rank)
+              u[e] = __ldcg(reinterpret_cast<const uint4*>(bp[e] + q)), v[e] = __ldcg(reinterpret_cast<const uint4*>(bp[e] + q + down[e]));
+          }
+#pragma unroll
+          for (int e = 0; e < PAIRS; ++e) {
+            const uint4 c = g < 3 ? *reinterpret_cast<const uint4*>(vs + r[e] * V_BYTES + v_at(g, q / 8 + t)) : make_uint4(0u, 0u, 0u, 0u);
+            mma16<false>(d[e], u[e].x, v[e].x, u[e].y, v[e].y, c.x, c.y);
+            mma16<false>(d[e], u[e].z, v[e].z, u[e].w, v[e].w, c.z, c.w);
           }
         }
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < PAIRS; ++e) {
-          const float both = a[e] + __shfl_xor_sync(0xffffffffu, a[e], 1);
-          if (half == 0 && bp[e]) sums[((i0 + e * cs * CW) / (8 * NT) * kw * 8 * NT + r[e]) * PP + lr] += both;
+        for (int e = 0; e < PAIRS; ++e) {  // the three terms' columns: two in lanes t = 0, one in t = 1
+          float lo = d[e][0] + d[e][1], hi = d[e][2] + d[e][3];
+          lo += __shfl_xor_sync(0xffffffffu, lo, 1), hi += __shfl_xor_sync(0xffffffffu, hi, 1);
+          float* at = sums + ((i0 + e * cs * CW) / (8 * NT) * kw * 8 * NT + r[e]) * PP + g;
+          if (t == 0 && bp[e]) at[0] += lo, at[8] += hi;
         }
       }
     }

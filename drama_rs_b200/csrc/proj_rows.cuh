@@ -51,17 +51,6 @@ struct Maps {
   CUtensorMap w, x;
 };
 
-// Four fp32 numbers as pairs of bf16 numbers in three terms (eight bits each, the third rounded).
-DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
-  float4 r = v;
-#pragma unroll
-  for (int l = 0; l < 3; ++l) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(r.x, r.y), c = __floats2bfloat162_rn(r.z, r.w);
-    b0[l] = *reinterpret_cast<const uint32_t*>(&a), b1[l] = *reinterpret_cast<const uint32_t*>(&c);
-    r = make_float4(r.x - __low2float(a), r.y - __high2float(a), r.z - __low2float(c), r.w - __high2float(c));
-  }
-}
-
 // After a wait that ran out: the copies and multiplications that this block has asked for end within the millisecond.
 DRB_DEV void linger() {
   for (int i = 0; i < 64; ++i) __nanosleep(16384);
@@ -206,7 +195,7 @@ __global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Ma
             const int r = r0 + 8 * i;
             if (r >= nc) break;
             uint32_t b0[3], b1[3];
-            split3(f[i], b0, b1);
+            pl::split3(f[i], b0, b1);
 #pragma unroll
             for (int l = 0; l < 3; ++l) *reinterpret_cast<uint2*>(xs + l * box + swz_off(r, k4 >> 1) + 8 * (k4 & 1)) = make_uint2(b0[l], b1[l]);
           }
