@@ -2,8 +2,9 @@
 //
 //   y_r = W x_r (+ res_r) + scale_a B_a (A_a x_r),  a = adapter_of[r]
 //
-// Two launches (one without adapters). v_r = scale_a A_a x_r: k_shrink, a warp a dot product, up to 64 rows, which may all have adapters of their own;
-// beyond, k_shrink_rows, sixteen rows a block on the tensor cores. Then the weights' stream, with the adapters' second half on its sums: k_proj up to 64 rows, k_proj_rows (tcgen05) beyond.
+// Two launches (one without adapters). v_r = scale_a A_a x_r: k_shrink, a warp a dot product, or k_shrink_rows, sixteen rows a block on
+// the tensor cores. Then the weights' stream, with the adapters' second half on its sums: k_proj behind the first, or, for many rows of few adapters or wide W (the rule and its
+// measurements: pr::many), k_proj_rows (tcgen05) behind the second.
 // Bound by the bytes of W and of the adapters hit for few rows, by the conversion of the codes for many.
 //
 // k_proj: 16-bit x meets the int8 codes, which both 16-bit types hold exactly, on mma.sync m16n8k16; a sum over the 128 inputs of a weight
@@ -15,8 +16,7 @@
 // runs: k_shrink lets this kernel in behind its own wait, so what came before k_shrink is complete.
 //
 // Queued (without adapters in brackets): 1 row of 2048 x 4096 7.2 us (5.4), 17 rows of 8192 x 2048 14.6 (8.8), 64 rows of 4096 x 2048 and as many adapters 17.6
-// (9.5). A step of 17 rows takes 0.8 us, of which mma.sync, conversion and reads of shared memory would each take half alone. 64 rows are two passes
-// here and would be one of k_proj_rows, which takes 11.3 us for 128 rows without adapters.
+// (9.5). A step of 17 rows takes 0.8 us, of which mma.sync, conversion and reads of shared memory would each take half alone. A pass takes up to 32 rows.
 #pragma once
 
 #include "common.cuh"
@@ -30,7 +30,6 @@ constexpr int SUB = 2048;                  // a step of a warp: 16 weight rows x
 constexpr int DEPTH = 3;
 constexpr int PP = 20;                     // floats between the columns of a tile of sums: writes of a warp meet no bank twice
 constexpr size_t SMEM_MAX = 232448, SMEM_TWO = 113 * 1024;  // up to the second, two blocks share a multiprocessor
-constexpr int TILE_ROWS = 64;              // up to so many rows: k_shrink and k_proj, beyond: k_shrink_rows and k_proj_rows
 
 struct Args {
   const int8_t* w;
@@ -560,8 +559,8 @@ static int launch_few(const Args& p, const DrbDevice& dev, cudaStream_t st) {
 }
 
 template <bool F16>
-static void launch_shrink(const Args& p, const DrbDevice& dev, cudaStream_t st) {
-  if (p.rows > TILE_ROWS) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
+static void launch_shrink(const Args& p, const DrbDevice& dev, bool many, cudaStream_t st) {
+  if (many) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
   else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), shrink_bytes(p.k), st, dev.pdl, p);
 }
 

@@ -77,6 +77,9 @@ def check(t, y, res=True):
 SHAPES = [(1, 2048, 4096, 1, 16), (1, 1, 128, 1, 8), (3, 17, 256, 2, 8), (8, 257, 2176, 5, 24), (9, 300, 512, 3, 64), (16, 128, 1024, 2, 16),
           (17, 1000, 2048, 4, 16), (32, 15, 640, 3, 8), (33, 2100, 1024, 7, 8), (64, 512, 2048, 64, 32), (65, 100, 8192, 2, 16), (5, 33, 8064, 2, 56),
           (130, 513, 384, 3, 40), (300, 256, 2048, 3, 64)]
+# wide enough for the tcgen05 form, from one tile of 16 rows to two of 80, and more than 64 rows of too many adapters for it
+SHAPES += [(10, 40000, 512, 1, 24), (24, 16400, 2048, 1, 16), (40, 8300, 2048, 2, 64), (60, 20000, 1024, 6, 8), (65, 9000, 640, 3, 40), (150, 5000, 2048, 2, 16),
+           (81, 20000, 256, 70, 8)]
 
 
 @pytest.mark.parametrize("x_type", [1, 2])
@@ -89,10 +92,10 @@ def test_against_the_definition(shape, x_type):
     check(t, run(t, res=False), res=False)
 
 
-@pytest.mark.parametrize("rows", [1, 12, 70])
+@pytest.mark.parametrize("rows,n", [(1, 200), (12, 200), (70, 200), (12, 30000), (70, 9000)])
 @pytest.mark.parametrize("adapters,rank", [(0, 0), (0, 16), (3, 0)])
-def test_the_projection_alone(rows, adapters, rank):
-    t = make(rows, rows, 200, 768, adapters, rank, 1, who=[0] * rows)
+def test_the_projection_alone(rows, n, adapters, rank):
+    t = make(rows, rows, n, 768, adapters, rank, 1, who=[0] * rows)
     check(t, run(t))
 
 
@@ -123,10 +126,10 @@ def test_a_row_of_nans_touches_no_other():
     assert torch.isnan(z[2]).all() and torch.equal(z[[0, 1, 3, 4, 5]], y[[0, 1, 3, 4, 5]])
 
 
-@pytest.mark.parametrize("rows", [6, 40, 70, 170])
-def test_a_broken_adapter_stays_with_its_own_rows(rows):
+@pytest.mark.parametrize("rows,n", [(6, 300), (40, 300), (70, 300), (170, 300), (33, 9000), (70, 9000), (170, 9000)])
+def test_a_broken_adapter_stays_with_its_own_rows(rows, n):
     who = [r % 4 - 1 for r in range(rows)]
-    t = make(rows, rows, 300, 512, 3, 16, 1, who=who)
+    t = make(rows, rows, n, 512, 3, 16, 1, who=who)
     y = run(t)
     t["b"][1, 7, 3] = float("nan")
     t["b"][1, 9, 4] = float("inf")
@@ -135,32 +138,32 @@ def test_a_broken_adapter_stays_with_its_own_rows(rows):
     sound = [r for r in range(rows) if who[r] < 1]
     assert torch.equal(z[sound], y[sound])
     one = [r for r in range(rows) if who[r] == 1]
-    kept = [c for c in range(300) if c not in (7, 9)]
+    kept = [c for c in range(n) if c not in (7, 9)]
     assert torch.isnan(z[one, 7]).all() and not torch.isfinite(z[one, 9]).any() and torch.equal(z[one][:, kept], y[one][:, kept])
     assert torch.isnan(z[[r for r in range(rows) if who[r] == 2]]).all()
 
 
-@pytest.mark.parametrize("rows", [20, 90])
-def test_two_calls_at_once_and_a_replay(rows):
+@pytest.mark.parametrize("rows,n", [(20, 700), (90, 700), (90, 9000)])
+def test_two_calls_at_once_and_a_replay(rows, n):
     """Two streams with scratch of their own; then one of them captured, behind itself, and replayed."""
     from drama_rs_b200.gpu import Graph
 
     l, sts = ffi.lib(), [Stream(), Stream()]
-    ts = [make(40 + i, rows + 3 * i, 700, 1024, 3, 16, 1 + i) for i in range(2)]
+    ts = [make(40 + i, rows + 3 * i, n, 1024, 3, 16, 1 + i) for i in range(2)]
     ref = [run(t) for t in ts]
     bufs, ys, vs = [], [], []
     for t, st in zip(ts, sts):
         bufs.append({name: up(t[name], st) for name in ("q", "s", "x", "a", "b", "scale", "who", "res")})
-        ys.append(DevBuf.zeros(t["dims"][0] * 700 * 4, st)), vs.append(DevBuf(t["dims"][0] * 16 * 4))
+        ys.append(DevBuf.zeros(t["dims"][0] * n * 4, st)), vs.append(DevBuf(t["dims"][0] * 16 * 4))
 
     def call(i):
-        b, (n, *_) = bufs[i], ts[i]["dims"]
-        launched(l.drb_proj_q8_lora(*(b[m].at(0) for m in ("q", "s", "x")), 1 + i, *(b[m].at(0) for m in ("a", "b", "scale", "who")), 3, 16, b["res"].at(0),
-                                    ys[i].at(0), vs[i].at(0), n, 700, 1024, sts[i].raw), "proj_q8_lora")
+        b, (m, *_) = bufs[i], ts[i]["dims"]
+        launched(l.drb_proj_q8_lora(*(b[a].at(0) for a in ("q", "s", "x")), 1 + i, *(b[a].at(0) for a in ("a", "b", "scale", "who")), 3, 16, b["res"].at(0),
+                                    ys[i].at(0), vs[i].at(0), m, n, 1024, sts[i].raw), "proj_q8_lora")
 
     def got(i):
-        n = ts[i]["dims"][0]
-        return torch.from_numpy(ys[i].download(np.float32, n * 700, sts[i]).reshape(n, 700))
+        m = ts[i]["dims"][0]
+        return torch.from_numpy(ys[i].download(np.float32, m * n, sts[i]).reshape(m, n))
 
     for _ in range(20):
         call(0), call(1)
