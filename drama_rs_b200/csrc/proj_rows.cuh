@@ -369,7 +369,8 @@ static int launch(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
 }
 
 // Which form: both sides' times in ns, from measurements of 1 to 300 rows, 2048 to 65536 outputs and 2048 to 8192 inputs (within a tenth or two).
-// The mma.sync form takes so many ns a million weights and pass, by its column tiles; a row's adapter costs it the row's outputs. The tcgen05 form takes
+// The mma.sync form takes so many ns a million weights and pass, by its column tiles, and a launch's start for every 32 passes, whose
+// clusters are about what is resident at once; a row's adapter costs it the row's outputs. The tcgen05 form takes
 // 450 ns for 128 inputs of a tile and 1250 for each different adapter of the tile's rows, every wave of tiles. The host does not know how many
 // meet in a tile: all that there are, up to 64 rows, which are likely to be as many requests; a quarter of them beyond, where neighbours are
 // likely to be of one. Measured, mma.sync / tcgen05, us: 8192 x 2048 24 rows 9.0 / 10.1, 48 rows 16.2 / 11.1; 32768 x 2048 24 rows 27 / 19; 2048 x 4096 64
@@ -379,7 +380,8 @@ static bool many(const pl::Args& p, const DrbDevice& dev, int nc, int row_tiles)
   const int nt = p.rows > 24 ? 4 : (p.rows + 7) / 8, passes = (p.rows + 8 * nt - 1) / (8 * nt);
   const long long tiles = (p.n + 127) / 128, blocks = tiles * row_tiles, waves = (blocks + dev.sms - 1) / dev.sms;
   const int most = p.rank > 0 ? (p.adapters < nc ? p.adapters : nc) : 0, met = p.rows <= 64 ? (most < p.rows ? most : p.rows) : (most + 3) / 4;
-  long long few = 3500 + PER_PASS[nt - 1] * passes * ((long long)p.n * p.k / 1000) / 1000, tc = 3000 + waves * (450 * (p.k / 128) + 1250 * met);
+  if (passes > 65535) return true;
+  long long few = 3500 * (1 + (passes - 1) / 32) + PER_PASS[nt - 1] * passes * ((long long)p.n * p.k / 1000) / 1000, tc = 3000 + waves * (450 * (p.k / 128) + 1250 * met);
   if (p.rank > 0) few += 3000 + (long long)p.n * (p.rows > 8 ? p.rows : 8) / 100, tc += 2500;
   return tc < few;
 }

@@ -12,6 +12,7 @@ import torch
 
 from drama_rs_b200 import ffi
 from drama_rs_b200.gpu import DevBuf, Stream, launched
+from tests.helpers import device_error_word
 
 pytestmark = pytest.mark.gpu
 TYPES = {0: torch.float32, 1: torch.bfloat16, 2: torch.float16}
@@ -131,3 +132,34 @@ def test_fp16_rows_are_clamped():
     i["pre"] = torch.full((512,), 1e6)
     _, h = run(**i, h_type=2)
     assert h.float().abs().max() == 65504.0 and torch.isfinite(h.float()).all()
+
+
+def test_offsets_past_32_bits():
+    """300,000 rows of 8192 (9.8 GB of x): zeros, but for the last row, which comes out as it does alone."""
+    rows, d = 300_000, 8192
+    st, l = Stream(), ffi.lib()
+    g = np.random.default_rng(5)
+    x1, w = g.standard_normal(d).astype(np.float32), (1 + 0.1 * g.standard_normal(d)).astype(np.float32)
+    o1 = (g.standard_normal(d).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)  # bf16
+    x, o, h = DevBuf.zeros(rows * d * 4, st), DevBuf.zeros(rows * d * 2, st), DevBuf.zeros(rows * d * 2, st)
+    dw = DevBuf.from_array(w, st)
+
+    def row(r):
+        x.upload(x1, st, r * d * 4)
+        o.upload(o1, st, r * d * 2)
+
+    def call(r0, count):
+        launched(l.drb_block_norms(o.at(r0 * d * 2), 1, dw.at(0), None, None, 0.5, x.at(r0 * d * 4), x.at(r0 * d * 4), dw.at(0), h.at(r0 * d * 2), 1, count, d,
+                                   1e-6, st.raw), "block_norms")
+
+    def got(r):
+        return x.download(np.float32, d, st, r * d * 4), h.download(np.uint16, d, st, r * d * 2)
+
+    row(rows - 1)
+    call(rows - 1, 1)
+    want = got(rows - 1)
+    row(rows - 1)
+    call(0, rows)
+    for a, b in zip(got(rows - 1), want):
+        assert np.array_equal(a, b)
+    assert not got(rows - 2)[0].any() and device_error_word() == 0

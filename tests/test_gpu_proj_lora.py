@@ -173,3 +173,39 @@ def test_two_calls_at_once_and_a_replay(rows, n):
     for _ in range(5):
         g.launch(sts[0]), call(1)
     assert torch.equal(got(0), ref[0]) and torch.equal(got(1), ref[1]) and device_error_word() == 0
+
+
+def test_more_rows_than_a_grid_has_passes():
+    """64 rows, over and over: every copy comes out as the first, and that one by the definition."""
+    rows, times = 64, 34000
+    t = make(1, rows, 3, 128, 1, 0, 1)
+    ref = dict(t)
+    st, l = Stream(), ffi.lib()
+    x = up(t["x"].repeat(times, 1), st)
+    q, s = up(t["q"], st), up(t["s"], st)
+    y = DevBuf.zeros(rows * times * 3 * 4, st)
+    launched(l.drb_proj_q8_lora(q.at(0), s.at(0), x.at(0), 1, None, None, None, None, 0, 0, None, y.at(0), None, rows * times, 3, 128, st.raw), "proj_q8_lora")
+    out = torch.from_numpy(y.download(np.float32, rows * times * 3, st).reshape(times, rows, 3))
+    check(ref, out[0], res=False)
+    assert (out == out[0]).all() and device_error_word() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_offsets_past_32_bits(rows):
+    """280,000 rows of W of 8192 inputs and 64 adapters: zeros, but for the last ones."""
+    n, k, adapters, rank, last = 280_000, 8192, 64, 64, 40
+    t = make(rows, rows, last, k, adapters, rank, 1, who=[adapters - 1 - (r % 2) * adapters for r in range(rows)])
+    st, l = Stream(), ffi.lib()
+    zeros = {"q": n * k, "s": n * (k // 128) * 2, "b": adapters * n * rank * 2}
+    b = {name: DevBuf.zeros(size, st) for name, size in zeros.items()}
+    bits = lambda a: (a.view(torch.int16) if a.dtype != torch.int8 else a).contiguous().numpy()
+    b["q"].upload(bits(t["q"]), st, (n - last) * k)
+    b["s"].upload(bits(t["s"]), st, (n - last) * (k // 128) * 2)
+    b["b"].upload(bits(t["b"][adapters - 1]), st, (adapters * n - last) * rank * 2)
+    b.update({name: up(t[name], st) for name in ("x", "a", "scale", "who")})
+    y, v = DevBuf.zeros(rows * n * 4, st), DevBuf(rows * rank * 4)
+    launched(l.drb_proj_q8_lora(*(b[a].at(0) for a in ("q", "s", "x")), 1, *(b[a].at(0) for a in ("a", "b", "scale", "who")), adapters, rank, None, y.at(0),
+                                v.at(0), rows, n, k, st.raw), "proj_q8_lora")
+    out = torch.from_numpy(y.download(np.float32, rows * n, st).reshape(rows, n))
+    check(t, out[:, n - last :].contiguous(), res=False)
+    assert (out[:, : n - last] == 0).all() and device_error_word() == 0
