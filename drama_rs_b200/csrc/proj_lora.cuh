@@ -49,15 +49,15 @@ DRB_DEV int adapter(const Args& p, int row) {  // -1: none
 }
 
 // ---- v = scale A x ------------------------------------------------------------------------------------------------------
-// A block: `groups` times eight ranks of one row, a warp one of each eight. Up to SK inputs of x and of two groups' rows of A come by asynchronous
-// copies at once: plain loads are few lines at a time beside the largest shared memory, and their registers kept blocks of k_proj off the multiprocessor.
-constexpr int SK = 4096, SK_GROUPS = 2048;  // inputs at once; up to so many a block may have several groups
-static int shrink_bytes(int k, int groups) { return 2 * (k < SK ? k : SK) * (groups > 1 ? 17 : 9); }
+// A block: eight ranks of one row, a warp each. Up to SK inputs of x and of the eight rows of A come by asynchronous copies at once: plain loads
+// are few lines at a time beside the largest shared memory, and their registers kept blocks of k_proj off the multiprocessor.
+constexpr int SK = 4096;
+static int shrink_bytes(int k) { return 9 * 2 * (k < SK ? k : SK); }
 template <bool F16>
-__global__ void __launch_bounds__(256, 6) k_shrink(Args p, int groups) {
+__global__ void __launch_bounds__(256, 6) k_shrink(Args p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  const int row = (int)blockIdx.x, warp = threadIdx.x >> 5, j0 = (int)blockIdx.y * 8 * groups + warp, lane = threadIdx.x & 31;
-  const int most = min(p.k, SK), ng = min(groups, (p.rank >> 3) - (int)blockIdx.y * groups);
+  const int row = (int)blockIdx.x, warp = threadIdx.x >> 5, j = (int)blockIdx.y * 8 + warp, lane = threadIdx.x & 31;
+  const int most = min(p.k, SK);
   const uint32_t xs = smem_u32(dyn), as = xs + 2 * most * (1 + warp);
   const uint16_t* xp = static_cast<const uint16_t*>(p.x) + (size_t)row * p.k;
   pdl_wait();
@@ -72,46 +72,32 @@ __global__ void __launch_bounds__(256, 6) k_shrink(Args p, int groups) {
     few::cp_wait<0>();
     return;
   }
-  const __nv_bfloat16* ap = p.a + ((size_t)ad * p.rank + j0) * p.k;
+  const __nv_bfloat16* ap = p.a + ((size_t)ad * p.rank + j) * p.k;
   const float scale = __ldcg(p.scale + ad);
   float acc[2] = {0.f, 0.f};
-  for (int k0 = 0; k0 < p.k; k0 += SK) {  // one chunk of inputs, or one group
+  for (int k0 = 0; k0 < p.k; k0 += SK) {
     if (k0 > 0) {
       __syncthreads();
       load_x(k0);
     }
     const int n = min(SK, p.k - k0) / 8;
-    auto issue = [&](int i) {
-      if (i < ng)
-        for (int q = lane; q < n; q += 32) few::cp16(as + (i & 1) * 16 * most + 16 * q, ap + (size_t)8 * i * p.k + k0 + 8 * q);
-      few::cp_commit();
-    };
-    issue(0);
-    issue(1);
-    for (int i = 0; i < ng; ++i) {
-      few::cp_wait<1>();
-      if (i == 0) __syncthreads();
-      else __syncwarp();
+    for (int i = lane; i < n; i += 32) few::cp16(as + 16 * i, ap + k0 + 8 * i);
+    few::cp_commit();
+    few::cp_wait<0>();
+    __syncthreads();
 #pragma unroll 4
-      for (int q = lane; q < n; q += 32) {
-        const uint4 xv = few::lds<uint4>(xs + 16 * q), av = few::lds<uint4>(as + (i & 1) * 16 * most + 16 * q);
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, aw[4] = {av.x, av.y, av.z, av.w};
+    for (int i = lane; i < n; i += 32) {
+      const uint4 xv = few::lds<uint4>(xs + 16 * i), av = few::lds<uint4>(as + 16 * i);
+      const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, aw[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          acc[0] = fmaf(widen16(xw[e] & 0xffffu, F16), widen16(aw[e] & 0xffffu, false), acc[0]);
-          acc[1] = fmaf(widen16(xw[e] >> 16, F16), widen16(aw[e] >> 16, false), acc[1]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        acc[0] = fmaf(widen16(xw[e] & 0xffffu, F16), widen16(aw[e] & 0xffffu, false), acc[0]);
+        acc[1] = fmaf(widen16(xw[e] >> 16, F16), widen16(aw[e] >> 16, false), acc[1]);
       }
-      if (k0 + SK >= p.k) {
-        const float sum = warp_sum(acc[0] + acc[1]);
-        if (lane == 0) p.v[(size_t)row * p.rank + j0 + 8 * i] = sum * scale;
-        acc[0] = acc[1] = 0.f;
-      }
-      __syncwarp();
-      issue(i + 2);
     }
   }
-  few::cp_wait<0>();
+  const float sum = warp_sum(acc[0] + acc[1]);
+  if (lane == 0) p.v[(size_t)row * p.rank + j] = sum * scale;
 }
 
 template <bool F16>
@@ -575,11 +561,7 @@ static int launch_few(const Args& p, const DrbDevice& dev, cudaStream_t st) {
 template <bool F16>
 static void launch_shrink(const Args& p, const DrbDevice& dev, bool many, cudaStream_t st) {
   if (many) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
-  else {
-    // a block of k_shrink keeps one of k_proj off its multiprocessor: beyond some twenty blocks, a row has one
-    const int groups = p.k <= SK_GROUPS && p.rows * (p.rank / 8) > 20 ? p.rank / 8 : 1;
-    drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8 / groups), dim3(256), shrink_bytes(p.k, groups), st, dev.pdl, p, groups);
-  }
+  else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), shrink_bytes(p.k), st, dev.pdl, p);
 }
 
 template <bool F16, int NT>
@@ -596,7 +578,7 @@ static cudaError_t configure_type() {
   if ((e = configure<F16, 4>()) != cudaSuccess) return e;
   if ((e = cudaFuncSetAttribute(k_shrink_rows<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SH_BYTES)) != cudaSuccess) return e;
   if ((e = drb_carveout(k_shrink_rows<F16>)) != cudaSuccess) return e;
-  if ((e = cudaFuncSetAttribute(k_shrink<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, shrink_bytes(SK, 1))) != cudaSuccess) return e;
+  if ((e = cudaFuncSetAttribute(k_shrink<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, shrink_bytes(SK))) != cudaSuccess) return e;
   return drb_carveout(k_shrink<F16>);
 }
 static cudaError_t configure_all() {

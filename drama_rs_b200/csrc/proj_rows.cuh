@@ -8,11 +8,11 @@
 // three bf16 terms, 24 bits; the accumulator joins with a factor of one. Bound by the conversion's issue slots, two instructions a
 // weight (bf16; fp16 one and a quarter) beside its loads and stores: 128 x 128 codes take a multiprocessor about 350 cycles, the
 // multiplications of nc = 80 take 160. Queued, 4096 x 2048, 300 rows: 12.4 us, with 3 adapters of rank 64 19.3; 8192 x 2048, 2048 rows: 133 us (0.52 PFLOP/s),
-// with adapters 159.
+// with adapters of rank 16 166.
 //
 // Roles, one block of 16 warps per multiprocessor, meeting on mbarriers, every wait bounded: 8 convert warps (two sets that take turns; a
 // thread the 128 codes of one weight row), 4 epilogue warps (a thread one weight row), one warp that issues the multiplications, one that issues the copies (tiled
-// TMA, 128-byte swizzle), one that looks at the rows' adapters. A block keeps its rows of x (blockIdx.y) and walks weight tiles.
+// TMA, 128-byte swizzle), one that looks at the rows' adapters. A block keeps its rows of x (blockIdx.y) and walks weight tiles (with adapters: one, see `launch`).
 #pragma once
 
 #include "moe_prefill_tc.cuh"
