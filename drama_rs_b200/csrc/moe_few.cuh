@@ -68,7 +68,7 @@ constexpr int MP = H / 64 + 1, DMP = I / 64 + 1;  // per 64 inputs, tokens apart
 constexpr int TOKEN_BYTES = TOKEN_PLANES + MP * 16;
 
 constexpr int DEPTH = 4;
-constexpr int CTL_BYTES = 3072, PLANES_BYTES = TOK * TOKEN_PLANES, META_BYTES = TOK * MP * 16, RING_BYTES = CW * DEPTH * SLOT, RED_BYTES = CW * 16 * 8 * 4;
+constexpr int CTL_BYTES = 3 * 1024, PLANES_BYTES = TOK * TOKEN_PLANES, META_BYTES = TOK * MP * 16, RING_BYTES = CW * DEPTH * SLOT, RED_BYTES = CW * 16 * 8 * 4;
 constexpr size_t SMEM_BYTES = CTL_BYTES + PLANES_BYTES + META_BYTES + RING_BYTES + RED_BYTES;
 static_assert(8 * MAX_TOK <= SHARED_BLOCKS * CW, "a warp for every eighth of a token");
 static_assert(SMEM_BYTES <= 232448 && 2 * 3 * TOK * DPITCH <= PLANES_BYTES && 2 * TOK * DMP * 16 <= META_BYTES, "shared memory");
