@@ -96,6 +96,12 @@ DRB_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Ahead of the arrival (or barrier) that hands a stage back to the copies: orders this thread's reads of shared memory before the writes of
+// bulk and tensor copies. A load has only been queued when the next instruction issues; an arrival does not stand in that queue, and
+// neither do the copies that it lets in, which belong to another proxy: without this (or a use of the values that were read) a load that is held up in
+// the queue finds the stage's next contents.
+DRB_DEV void reads_before_copies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 DRB_DEV bool mbar_try_wait(uint64_t* bar, unsigned parity) {
   unsigned ok;
   asm volatile(

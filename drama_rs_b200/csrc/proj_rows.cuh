@@ -146,10 +146,6 @@ __global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Ma
           uint4 v[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(raw + r * RAW_BYTES + swz_off(row, 4 * half + j));
-          if (half == 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl.rawempty[r]);
-          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             pl::widen_codes<F16>(v[j].x, o[8 * j], o[8 * j + 1]);
@@ -163,6 +159,11 @@ __global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Ma
           }
           tmem_st32(ta + 64 * s + 32 * half, o);
         }
+        // The stage goes back behind the stores that use its last codes: an arrival between the loads and their use let the stage's next codes in ahead of
+        // loads that stood in the queue behind the other set's of an adapter's B (32 lines each; half of all calls of 280,000 x 8192 with adapters)
+        reads_before_copies();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.rawempty[r]);
       } else {
         // an adapter: 64 ranks (zeros behind the last) of B's rows, and v
         const int ad = ctl.diff[g - groups], wr = (first + t * step) * 128 + row;
