@@ -8,11 +8,11 @@
 // three bf16 terms, 24 bits; the accumulator joins with a factor of one. Bound by the conversion's issue slots, two instructions a
 // weight (bf16; fp16 one and a quarter) beside its loads and stores: 128 x 128 codes take a multiprocessor about 350 cycles, the
 // multiplications of nc = 80 take 160. Queued, 4096 x 2048, 300 rows: 12.4 us, with 3 adapters of rank 64 19.3; 8192 x 2048, 2048 rows: 133 us (0.52 PFLOP/s),
-// with adapters of rank 16 166.
+// with three adapters of rank 16 159 (one tile a block: 168).
 //
 // Roles, one block of 16 warps per multiprocessor, meeting on mbarriers, every wait bounded: 8 convert warps (two sets that take turns; a
 // thread the 128 codes of one weight row), 4 epilogue warps (a thread one weight row), one warp that issues the multiplications, one that issues the copies (tiled
-// TMA, 128-byte swizzle), one that looks at the rows' adapters. A block keeps its rows of x (blockIdx.y) and walks weight tiles (with adapters: one, see `launch`).
+// TMA, 128-byte swizzle), one that looks at the rows' adapters. A block keeps its rows of x (blockIdx.y) and walks weight tiles.
 #pragma once
 
 #include "moe_prefill_tc.cuh"
@@ -364,9 +364,7 @@ static int launch(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
   if (!e) e = map_2d(&maps.x, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.x, p.k, p.rows, (uint64_t)p.k * 2, 64, nc);
   if (e) return e;
   if (p.rank > 0) pl::launch_shrink<F16>(p, dev, true, st);
-  // Without adapters a block walks over tiles; with them it has one. Behind an adapter's stretch the next tile's first 128 inputs came out with codes of its fifth
-  // ones now and then (280,000 x 8192, one tile in fifteen a block; the cause was not found): with one tile nothing comes behind the adapters.
-  const int each = p.rank > 0 ? tiles : dev.sms / passes;
+  const int each = dev.sms / passes;
   drb_launch(k_proj_rows<F16>, dim3(each < 1 ? 1 : each < tiles ? each : tiles, passes), dim3(THREADS), smem_bytes(nc), st, dev.pdl, maps, p, nc, tiles);
   return 0;
 }
@@ -374,7 +372,7 @@ static int launch(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
 // Which form: both sides' times in ns, from measurements of 1 to 300 rows, 2048 to 65536 outputs and 2048 to 8192 inputs (within a tenth or two).
 // The mma.sync form takes so many ns a million weights and pass, by its column tiles, and a launch's start for every 32 passes, whose
 // clusters are about what is resident at once; a row's adapter costs it the row's outputs. The tcgen05 form takes
-// 450 ns for 128 inputs of a tile and 1250 for each different adapter of the tile's rows, every wave of tiles, with adapters and a start of its own. The host does not know how many
+// 450 ns for 128 inputs of a tile and 1250 for each different adapter of the tile's rows, every wave of tiles. The host does not know how many
 // meet in a tile: all that there are, up to 64 rows, which are likely to be as many requests; a quarter of them beyond, where neighbours are
 // likely to be of one. Measured, mma.sync / tcgen05, us: 8192 x 2048 24 rows 9.0 / 10.1, 48 rows 16.2 / 11.1; 32768 x 2048 24 rows 27 / 19; 2048 x 4096 64
 // rows 10.9 / 18.7; 8192 x 2048, 48 rows of 8 adapters 25.3 / 22.7, of 16 25.4 / 34.9.
@@ -385,7 +383,7 @@ static bool many(const pl::Args& p, const DrbDevice& dev, int nc, int row_tiles)
   const int most = p.rank > 0 ? (p.adapters < nc ? p.adapters : nc) : 0, met = p.rows <= 64 ? (most < p.rows ? most : p.rows) : (most + 3) / 4;
   if (passes > 65535) return true;
   long long few = 3500 * (1 + (passes - 1) / 32) + PER_PASS[nt - 1] * passes * ((long long)p.n * p.k / 1000) / 1000, tc = 3000 + waves * (450 * (p.k / 128) + 1250 * met);
-  if (p.rank > 0) few += 3000 + (long long)p.n * (p.rows > 8 ? p.rows : 8) / 100, tc += 2500 + 3000 * (waves - 1);
+  if (p.rank > 0) few += 3000 + (long long)p.n * (p.rows > 8 ? p.rows : 8) / 100, tc += 2500;
   return tc < few;
 }
 

@@ -34,7 +34,7 @@ def takes_tcgen05(rows, n, k, adapters, rank):
     tc = 3000 + waves * (450 * (k // 128) + 1250 * met)
     if rank:
         few += 3000 + n * max(rows, 8) // 100
-        tc += 2500 + 3000 * (waves - 1)
+        tc += 2500
     return tc < few
 
 
@@ -112,3 +112,21 @@ ALONE = [(16, 60_001, 768), (80, 60_001, 768), (16, 75_700, 8192), (80, 57_000, 
 def test_several_tiles_without_adapters(rows, n, k, x_type):
     assert takes_tcgen05(rows, n, k, 0, 0) and tiles_a_block(rows, n) > 3
     many_calls(Case(rows + n + k, rows, n, k, x_type), 100)
+
+
+# With none, one, two and three different adapters among a tile's rows (an odd number of them hands every stage of the codes from one set of convert warps
+# to the other at a tile's end), ranks from the smallest to the largest, rows of one adapter behind one another and mixed
+BESIDE = [(16, 75_700, 768, 1, 8), (16, 75_700, 8192, 1, 16), (16, 75_700, 8192, 2, 64), (16, 75_700, 8192, 3, 24), (80, 60_001, 768, 1, 64),
+          (80, 60_001, 768, 2, 16), (80, 60_001, 768, 3, 40), (80, 57_000, 8192, 1, 16), (80, 57_000, 8192, 2, 8), (80, 57_000, 8192, 3, 64),
+          (150, 57_003, 2048, 3, 16), (300, 40_000, 1024, 9, 32)]
+
+
+@pytest.mark.parametrize("x_type", [1, 2])
+@pytest.mark.parametrize("rows,n,k,adapters,rank", BESIDE)
+def test_several_tiles_with_adapters(rows, n, k, adapters, rank, x_type):
+    assert takes_tcgen05(rows, n, k, adapters, rank) and tiles_a_block(rows, n) > 3
+    rng = np.random.default_rng(rows + n + k + rank)
+    mixed = rng.integers(-1, adapters, rows).tolist()
+    runs = sorted(mixed)  # neighbours of one adapter: many rows' tiles differ in how many they meet
+    for who in ([-1] * rows, [0] * rows, mixed, runs):
+        many_calls(Case(rows + n + k, rows, n, k, x_type, adapters, rank, who), 100)
