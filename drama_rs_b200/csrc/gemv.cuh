@@ -62,7 +62,7 @@ struct Shape {
   static constexpr int PITCH = SEG + 64;                // bytes between rows in a stage: rows r and r + 1 on different banks
   static constexpr int SROW = K / GROUP * 2;            // bytes of scales per row
   static constexpr bool S_COPY = SROW >= 16;            // bulk copies need 16-byte granules
-  static constexpr int S_SLOTS = S_COPY ? (NSEG > 1 ? 2 : 3) : 0;  // see the producer
+  static constexpr int S_SLOTS = S_COPY ? (NSEG > 2 ? 2 : 3) : 0;  // see the producer
   static constexpr int STAGE_BYTES = ROWS * PITCH;
   static constexpr int WARP_BYTES = 2 * BATCH * 4;      // per warp: limbs on their way to the operand layout, then two batches of partial sums
   static constexpr size_t BYTES = 512 + (size_t)STAGES * STAGE_BYTES + S_SLOTS * ROWS * SROW + CW * WARP_BYTES;
@@ -87,7 +87,7 @@ DRB_DEV void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t
 template <int K, int U>
 __global__ void __launch_bounds__(THREADS, 2)
     k_gemv(const int8_t* __restrict__ W, const __half* __restrict__ S, const float* __restrict__ x, const float* res, float* y, int N,
-           const float* __restrict__ nw, float eps, const char* pf, size_t pf_bytes, unsigned pf_skip, unsigned sms) {
+           const float* __restrict__ nw, float eps, const char* pf, size_t pf_bytes, unsigned pf_skip, unsigned sms, uint32_t none) {
   using P = Shape<K, U>;
   constexpr int STAGES = P::STAGES, NSEG = P::NSEG, KW = P::KW, RS = P::RS, ROWS = P::ROWS, SEG = P::SEG, PITCH = P::PITCH, SROW = P::SROW;
   constexpr int SLOTS = P::S_SLOTS ? P::S_SLOTS : 1;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (warp == CW) {
     // ---------------- producer: weights are constants, so copies start before the dependency wait. A tile's scales come with its
     // first stage into one of S_SLOTS slots; the stage STAGES requests back has been read by then, so the slot's last tile is done.
-    static_assert(P::S_SLOTS == 0 || P::S_SLOTS * NSEG >= STAGES + NSEG - 1, "scale slots");
+    static_assert(P::S_SLOTS == 0 || P::S_SLOTS * NSEG >= STAGES + NSEG - 1 + (NSEG == 2 ? 2 : 0), "scale slots");
     if (elect_one()) {
       int s = 0;
       uint32_t par = 1;  // every stage starts free
@@ -152,9 +152,9 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint32_t par = 0;
   uint4 v0, v1, w0, w1;  // rows g and g + 8 of the tile, two pieces each
   __half sc0 = __half(), sc1 = __half();
-  auto release = [&]() {
+  auto release = [&](uint32_t word) {
     __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.empty[s]);
+    if (lane == 0) mbar_arrive_behind(word, none, &ctl.empty[s]);
     if (++s == STAGES) s = 0, par ^= 1u;
   };
   auto operand = [&]() { return ring + s * P::STAGE_BYTES + (sub * 16 + g) * PITCH + kw * GROUP + 16 * t4; };
@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(THREADS, 2)
       const unsigned char* sp = scales + (t % SLOTS * ROWS + sub * 16 + g) * SROW + 2 * (q * KW + kw);
       sc0 = *reinterpret_cast<const __half*>(sp), sc1 = *reinterpret_cast<const __half*>(sp + 8 * SROW);
     }
-    if (EARLY) release();
+    // With two segments a row the scales' next copy is let in a whole tile later, behind their use
+    if (EARLY) release(v0.x ^ w0.x ^ v1.x ^ w1.x ^ (P::S_COPY && NSEG == 1 ? (uint32_t)(__half_as_ushort(sc0) ^ __half_as_ushort(sc1)) : 0u));
   };
   // The norm weights are brought as far as L2 before the input may be read (they may be the work of the launch before).
   float4 wv[NSEG], xv[NSEG];
@@ -259,13 +260,13 @@ __global__ void __launch_bounds__(THREADS, 2)
         mma_s8(c, v0.z, w0.z, v0.w, w0.w, bf[q][2], bf[q][3]);
         const unsigned char* rp = operand() + 64;
         v0 = *reinterpret_cast<const uint4*>(rp), w0 = *reinterpret_cast<const uint4*>(rp + 8 * PITCH);
-        release();
         mma_s8(c, v0.x, w0.x, v0.y, w0.y, bf[q][4], bf[q][5]);
         mma_s8(c, v0.z, w0.z, v0.w, w0.w, bf[q][6], bf[q][7]);
       }
       // |a limb's sum| <= 128 * 128 * 64 = 2^20: limb + 128 * next limb stays an exact integer
       a0 = fmaf(__half2float(sc0) * delta[q], (float)((c[0] + e[0]) + ((c[1] + e[1]) << 7)), a0);
       a1 = fmaf(__half2float(sc1) * delta[q], (float)((c[2] + e[2]) + ((c[3] + e[3]) << 7)), a1);
+      if (!EARLY) release(__float_as_uint(a0) ^ __float_as_uint(a1));
       if (EARLY) {
         if (q + 1 < NSEG) load(t, q + 1);
         else if (t + 1 < ntiles) load(t + 1, 0);
@@ -314,7 +315,7 @@ int launch(const int8_t* W, const __half* S, const float* x, const float* res, f
   if (!dev.ready) return -2;
   if (N <= 0) return 0;
   drb_launch(k_gemv<K, U>, dim3(N < dev.sms ? N : dev.sms), dim3(THREADS), Shape<K, U>::BYTES, st, dev.pdl, W, S, x, res, y, N, nw, eps, pf, pf_bytes,
-             dev.pdl ? HINT_SKIP : 0u, (unsigned)dev.sms);
+             dev.pdl ? HINT_SKIP : 0u, (unsigned)dev.sms, 0u);
   return 0;
 }
 
@@ -345,7 +346,7 @@ DRB_DEV void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memor
 
 __global__ void __launch_bounds__(THREADS, 2)
     k_gemv(const __nv_bfloat16* __restrict__ W, const float* __restrict__ x, float* __restrict__ y, int N, const float* __restrict__ nw, float eps,
-           const char* pf, size_t pf_bytes, unsigned pf_skip, unsigned sms) {
+           const char* pf, size_t pf_bytes, unsigned pf_skip, unsigned sms, uint32_t none) {
   extern __shared__ __align__(128) unsigned char dyn[];
   Ctl& ctl = *reinterpret_cast<Ctl*>(dyn);
   float4* xs4 = reinterpret_cast<float4*>(dyn + 512);
@@ -428,11 +429,11 @@ __global__ void __launch_bounds__(THREADS, 2)
         a1 = dot8_bf16(*reinterpret_cast<const uint4*>(rowp + 16 * (lane + 32 * (i + 1))), xp + (i + 1) * 4, a1);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl.empty[s]);
     float p0, p1, p2, p3;
     unpack2(a0, p0, p1);
     unpack2(a1, p2, p3);
+    __syncwarp();
+    if (lane == 0) mbar_arrive_behind(__float_as_uint(p0) ^ __float_as_uint(p2), none, &ctl.empty[s]);
     const float d = warp_sum((p0 + p1) + (p2 + p3));
     if (lane == 0 && row < u1) y[row] = d * inv;
   }
@@ -492,6 +493,6 @@ extern "C" int dr_gemv_bf16(const __nv_bfloat16* W, const float* x, float* y, in
   if (!dev.ready) return -2;
   if (N <= 0) return 0;
   drb_launch(k_gemv, dim3(N < dev.sms ? N : dev.sms), dim3(THREADS), BYTES, st, dev.pdl, W, x, y, N, nw, eps, pf, pf_bytes,
-             dev.pdl ? gemv::HINT_SKIP : 0u, (unsigned)dev.sms);
+             dev.pdl ? gemv::HINT_SKIP : 0u, (unsigned)dev.sms, 0u);
   return 0;
 }

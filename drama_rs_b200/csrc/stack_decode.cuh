@@ -677,6 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           v[2 * i + 1] = u0.x * x0.delta * dot32_q4_i(ur[lane], x0, 0) + u0.y * X0 + u1.x * x1.delta * dot32_q4_i(ur[32 + lane], x1, 0) + u1.y * X1;
         }
       }
+      reads_before_copies();
       bar_arrive<THREADS>(BAR_GU);  // nothing of the stage is read after this point
       // Fold the four per-lane sums into one reduction.
       const bool hi16 = lane & 16, hi8 = lane & 8;
@@ -757,6 +758,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           s_sh = ssc * sq.delta * dot16_q8_i(*reinterpret_cast<const uint4*>(dst + TOPK * D_EXPERT + (size_t)warp * I + 16 * lane), sq, 0);
         }
       }
+      reads_before_copies();
       bar_arrive<THREADS>(BAR_DN);  // nothing of the stage is read after this point
       {
         // Fold the four sums (each to be reduced over the 8 lanes of a row group) into one reduction.

@@ -31,12 +31,25 @@ def between(text: str, read: str, release: str) -> list[str]:
 
 @pytest.mark.parametrize("file,read,release,places", [("proj_rows.cuh", "(raw + r * RAW_BYTES", "mbar_arrive(&ctl.rawempty[r])", 1),
                                                       ("moe_prefill_tc.cuh", "lds128(xa", "mbar_arrive(&ctl.rawempty[rr.i])", 1),
-                                                      ("moe_prefill_tc.cuh", "(xp + piece(", "mbar_arrive(&ctl.rawempty[sa])", 1)])
+                                                      ("moe_prefill_tc.cuh", "(xp + piece(", "mbar_arrive(&ctl.rawempty[sa])", 1),
+                                                      ("stack_decode.cuh", "dot32_q4_i(gr[lane]", "bar_arrive<THREADS>(BAR_GU)", 2),
+                                                      ("stack_decode.cuh", "(dst + TOPK * D_EXPERT + (size_t)warp", "bar_arrive<THREADS>(BAR_DN)", 1)])
 def test_a_stage_goes_back_behind_the_use_of_its_reads(file, read, release, places):
     texts = between(source(file), read, release)
     assert len(texts) == places
     for t in texts:
         assert any(o in t for o in ORDERED), t
+
+
+def test_a_gemvs_stage_goes_back_by_an_arrival_that_waits_for_the_reads():
+    """There the address of the arrival is made from what was read: from all pieces of a row, and from the scales unless the slot that they lie in is
+    filled again a tile later."""
+    text = source("gemv.cuh")
+    assert "mbar_arrive(&ctl.empty" not in text and text.count("mbar_arrive_behind(") == 2
+    calls = re.findall(r" release\((.*)\);", text)
+    assert len(calls) == 2 and all(w in calls[0] for w in ("v0.x", "v1.x", "w0.x", "w1.x", "sc0", "sc1")), calls
+    assert all(w in calls[1] for w in ("a0", "a1"))
+    assert "+ (NSEG == 2 ? 2 : 0)" in text  # the slots' count, by which two segments do without the scales
 
 
 def test_the_scan_sees_an_arrival_between_the_reads_and_their_use():
