@@ -407,14 +407,26 @@ class MoeBatchDecoder:
         return self.row.get(self.x).reshape(self.streams, self.hidden)
 
 
+def _holds(what: str, buf, nbytes: int) -> None:
+    """Refuses a buffer that the kernels would read or write past its end."""
+    if buf is not None and buf.nbytes < nbytes:
+        raise ValueError(f"{what} has {buf.nbytes} bytes where the call needs {nbytes}")
+
+
 def project_rows(w: Q8, x, x_type: int, y, rows: int, st: Stream, adapters: Adapters | None = None, adapter_of=None, v=None, res=None) -> None:
     """y [rows, n] f32 = x W^T (+ res) with each row's adapter beside it (drb_proj_q8_lora). x: 16-bit rows of x_type (1: bf16, 2: fp16);
-    adapter_of: int32 [rows], out of range = none; v: scratch f32 [rows, rank]. All are device buffers; y may be res."""
+    adapter_of: int32 [rows], out of range = none; v: scratch f32 [rows, rank]. All are device buffers; y may be res. A buffer that is too small is a
+    ValueError."""
     at = lambda b: b.at(0) if b is not None else NULL
     q, s = w.rows(0)
-    if adapters is not None:
-        assert (adapters.n, adapters.k) == (w.n, w.k) and adapter_of is not None and v is not None
     a = adapters
+    _holds("w.q", w.q, w.n * w.k), _holds("w.s", w.s, w.n * (w.k // 128) * 2)
+    _holds("x", x, rows * w.k * 2), _holds("y", y, rows * w.n * 4), _holds("res", res, rows * w.n * 4)
+    if a is not None:
+        if (a.n, a.k) != (w.n, w.k) or adapter_of is None or v is None:
+            raise ValueError(f"adapters of {a.n} x {a.k} for a projection of {w.n} x {w.k}, or no adapter_of or no v")
+        _holds("adapters.a", a.a, a.count * a.rank * a.k * 2), _holds("adapters.b", a.b, a.count * a.n * a.rank * 2)
+        _holds("adapters.scale", a.scale, a.count * 4), _holds("adapter_of", adapter_of, rows * 4), _holds("v", v, rows * a.rank * 4)
     launched(ffi.lib().drb_proj_q8_lora(q, s, x.at(0), x_type, at(a and a.a), at(a and a.b), at(a and a.scale), at(adapter_of if a else None),
                                         a.count if a else 0, a.rank if a else 0, at(res), y.at(0), at(v if a else None), rows, w.n, w.k, st.raw),
              "proj_q8_lora")
@@ -423,7 +435,12 @@ def project_rows(w: Q8, x, x_type: int, y, rows: int, st: Stream, adapters: Adap
 def block_norms(o, o_type: int, x, x_out, rows: int, d: int, st: Stream, post_w=None, gate=None, scale=None, alpha: float = 1.0, pre_w=None, h=None,
                 h_type: int = 1, eps: float = 1e-6) -> None:
     """x_out = alpha x + sigmoid(gate) scale rmsnorm(o, post_w), h = rmsnorm(x_out, pre_w) (drb_block_norms); device buffers, types 0: f32, 1: bf16,
-    2: fp16; parts that are None are left out."""
+    2: fp16; parts that are None are left out. A buffer that is too small is a ValueError."""
     at = lambda b: b.at(0) if b is not None else NULL
+    size = {0: 4, 1: 2, 2: 2}  # of other types the call refuses
+    _holds("o", o, rows * d * size.get(o_type, 0)), _holds("x", x, rows * d * 4), _holds("x_out", x_out, rows * d * 4)
+    _holds("post_w", post_w, d * 4), _holds("gate", gate, rows * 4), _holds("scale", scale, d * 4), _holds("pre_w", pre_w, d * 4)
+    if pre_w is not None:
+        _holds("h", h, rows * d * size.get(h_type, 0))
     launched(ffi.lib().drb_block_norms(o.at(0), o_type, at(post_w), at(gate), at(scale), alpha, x.at(0), x_out.at(0), at(pre_w), at(h), h_type, rows, d, eps,
                                        st.raw), "block_norms")
