@@ -507,7 +507,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
 }
 
 // Clusters of cs blocks that are resident at once, with one block a multiprocessor and with two: a property of the device, asked once.
-static int g_clusters[32][2][4];
+constexpr int MAX_DEVICES = 32;
+static int g_clusters[MAX_DEVICES][2][4];
 
 // The rows of x decide NT, up to 32 a pass. Blocks of a cluster (cs) and warps of a block (kw) share K. Of all splits whose slice of x fits, the one
 // with the least work on a warp's way (of equals the widest cluster, whose blocks read least of x): batches of tiles, each (in halves of a step) its steps and about three steps of a
@@ -515,7 +516,7 @@ static int g_clusters[32][2][4];
 template <bool F16, int NT>
 static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   int d = 0;
-  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 32) return -2;
+  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= MAX_DEVICES) return -2;
   const int groups = p.k / 128, mt = (p.n + 15) / 16, passes = (p.rows + 8 * NT - 1) / (8 * NT);
   int cs = 8, kw = 1, clusters = 1;
   long long least = -1;
@@ -586,7 +587,7 @@ static cudaError_t configure_all() {
   if (e != cudaSuccess || (e = configure_type<true>()) != cudaSuccess) return e;
   int d = 0;
   if ((e = cudaGetDevice(&d)) != cudaSuccess) return e;
-  if (d < 0 || d >= 32) return cudaErrorInvalidDevice;
+  if (d < 0 || d >= MAX_DEVICES) return cudaErrorInvalidDevice;
   for (int two = 0; two < 2; ++two)
     for (int lg = 0; lg < 4; ++lg) {
       cudaLaunchConfig_t cfg = {};

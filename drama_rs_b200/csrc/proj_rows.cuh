@@ -387,10 +387,17 @@ static bool many(const pl::Args& p, const DrbDevice& dev, int nc, int row_tiles)
   return tc < few;
 }
 
+// Whether k_proj_rows was compiled with the registers that its roles share out. Where it was not, the mma.sync form takes every call, up to as many rows as a grid
+// has passes, and nothing else of the library is touched.
+static bool g_fits[pl::MAX_DEVICES];
+
 template <bool F16>
 static int launch_any(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= pl::MAX_DEVICES) return -2;
   const int ny = (p.rows + MAX_C - 1) / MAX_C, nc = ((p.rows + ny - 1) / ny + 15) / 16 * 16;
-  if (many(p, dev, nc, (p.rows + nc - 1) / nc)) return launch<F16>(p, dev, st);
+  if (g_fits[d] && many(p, dev, nc, (p.rows + nc - 1) / nc)) return launch<F16>(p, dev, st);
+  if (p.rows > 65535 * 32) return -1;
   if (p.rank > 0) pl::launch_shrink<F16>(p, dev, false, st);
   return pl::launch_few<F16>(p, dev, st);
 }
@@ -401,7 +408,10 @@ static cudaError_t configure_all() {
   if ((e = cudaFuncSetAttribute(k_proj_rows<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(MAX_C))) != cudaSuccess) return e;
   cudaFuncAttributes a, b;  // with fewer registers at the launch than the shares add up to the warps would wait for the rest
   if ((e = cudaFuncGetAttributes(&a, k_proj_rows<true>)) != cudaSuccess || (e = cudaFuncGetAttributes(&b, k_proj_rows<false>)) != cudaSuccess) return e;
-  if (a.numRegs < LAUNCH_REGS || b.numRegs < LAUNCH_REGS) return cudaErrorInvalidConfiguration;
+  int d = 0;
+  if ((e = cudaGetDevice(&d)) != cudaSuccess) return e;
+  if (d < 0 || d >= pl::MAX_DEVICES) return cudaErrorInvalidDevice;
+  g_fits[d] = a.numRegs >= LAUNCH_REGS && b.numRegs >= LAUNCH_REGS;
   if ((e = drb_carveout(k_proj_rows<true>)) != cudaSuccess) return e;
   return drb_carveout(k_proj_rows<false>);
 }
