@@ -506,32 +506,53 @@ __global__ void __launch_bounds__(THREADS, 2) k_proj(Args p, Split sp) {
   few::cp_wait<0>();
 }
 
+template <bool F16>
+static void launch_shrink(const Args& p, const DrbDevice& dev, bool many, cudaStream_t st) {
+  if (many) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
+  else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), shrink_bytes(p.k), st, dev.pdl, p);
+}
+
 // Clusters of cs blocks that are resident at once, with one block a multiprocessor and with two: a property of the device, asked once.
 constexpr int MAX_DEVICES = 32;
 static int g_clusters[MAX_DEVICES][2][4];
 
 // The rows of x decide NT, up to 32 a pass. Blocks of a cluster (cs) and warps of a block (kw) share K. Of all splits whose slice of x fits, the one
 // with the least work on a warp's way (of equals the widest cluster, whose blocks read least of x): batches of tiles, each (in halves of a step) its steps and about three steps of a
-// batch's end, which grows with the slices whose sums meet there.
-template <bool F16, int NT>
-static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
-  int d = 0;
-  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= MAX_DEVICES) return -2;
-  const int groups = p.k / 128, mt = (p.n + 15) / 16, passes = (p.rows + 8 * NT - 1) / (8 * NT);
-  int cs = 8, kw = 1, clusters = 1;
+// batch's end, which grows with the slices whose sums meet there. `resident`: clusters of 1, 2, 4
+// and 8 blocks that the device holds at once, [0] with one block a multiprocessor, [1] with two; 0: it runs none of that width.
+struct Plan {
+  int cs, kw, clusters;  // clusters 0: no width runs
+};
+template <int NT>
+static Plan plan(const int (&resident)[2][4], int rows, int n, int k) {
+  const int groups = k / 128, mt = (n + 15) / 16, passes = (rows + 8 * NT - 1) / (8 * NT);
+  Plan best = {0, 0, 0};
   long long least = -1;
   for (int lg = 0; lg < 4 && 1 << lg <= groups; ++lg) {
     const int slice = (groups + (1 << lg) - 1) >> lg;
     const size_t bytes = Shape<NT>::bytes(128 * slice);
     if (bytes > SMEM_MAX) continue;
-    const int avail = g_clusters[d][bytes <= SMEM_TWO][lg] / passes;
+    const int all = resident[bytes <= SMEM_TWO][lg], avail = all / passes;
+    if (all < 1) continue;
     for (int w = 1; w <= 4 && w <= slice; w *= 2) {
       const int need = (int)(((long long)mt * w + CW - 1) / CW), have = avail < 1 ? 1 : avail < need ? avail : need;
-      const int waves = avail < 1 ? (passes + g_clusters[d][bytes <= SMEM_TWO][lg] - 1) / g_clusters[d][bytes <= SMEM_TWO][lg] : 1;
+      const int waves = avail < 1 ? (passes + all - 1) / all : 1;
       const long long cost = (long long)waves * ((need + have - 1) / have) * (2 * ((slice + w - 1) / w) + 6 + w * (1 << lg) / 2);
-      if (least < 0 || cost <= least) least = cost, cs = 1 << lg, kw = w, clusters = have;
+      if (least < 0 || cost <= least) least = cost, best = {1 << lg, w, have};
     }
   }
+  return best;
+}
+
+template <bool F16, int NT>
+static int launch(const Args& p, const DrbDevice& dev, cudaStream_t st) {
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= MAX_DEVICES) return -2;
+  const int groups = p.k / 128, mt = (p.n + 15) / 16, passes = (p.rows + 8 * NT - 1) / (8 * NT);
+  const Plan pn = plan<NT>(g_clusters[d], p.rows, p.n, p.k);
+  if (pn.clusters == 0) return -1;
+  const int cs = pn.cs, kw = pn.kw, clusters = pn.clusters;
+  if (p.rank > 0) launch_shrink<F16>(p, dev, false, st);
   const size_t smem = Shape<NT>::bytes(128 * ((groups + cs - 1) / cs));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * cs, passes);
@@ -557,12 +578,6 @@ static int launch_few(const Args& p, const DrbDevice& dev, cudaStream_t st) {
   if (p.rows <= 16) return launch<F16, 2>(p, dev, st);
   if (p.rows <= 24) return launch<F16, 3>(p, dev, st);
   return launch<F16, 4>(p, dev, st);
-}
-
-template <bool F16>
-static void launch_shrink(const Args& p, const DrbDevice& dev, bool many, cudaStream_t st) {
-  if (many) drb_launch(k_shrink_rows<F16>, dim3((p.rows + 15) / 16, p.rank / 8), dim3(256), SH_BYTES, st, dev.pdl, p);
-  else drb_launch(k_shrink<F16>, dim3(p.rows, p.rank / 8), dim3(256), shrink_bytes(p.k), st, dev.pdl, p);
 }
 
 template <bool F16, int NT>
@@ -596,7 +611,7 @@ static cudaError_t configure_all() {
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = 1 << lg, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr, cfg.numAttrs = 1;
-      if ((e = cudaOccupancyMaxActiveClusters(&g_clusters[d][two][lg], k_proj<true, 4>, &cfg)) != cudaSuccess) return e;
+      if (cudaOccupancyMaxActiveClusters(&g_clusters[d][two][lg], k_proj<true, 4>, &cfg) != cudaSuccess) g_clusters[d][two][lg] = 0, cudaGetLastError();
     }
   return cudaSuccess;
 }

@@ -398,7 +398,6 @@ static int launch_any(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) 
   const int ny = (p.rows + MAX_C - 1) / MAX_C, nc = ((p.rows + ny - 1) / ny + 15) / 16 * 16;
   if (g_fits[d] && many(p, dev, nc, (p.rows + nc - 1) / nc)) return launch<F16>(p, dev, st);
   if (p.rows > 65535 * 32) return -1;
-  if (p.rank > 0) pl::launch_shrink<F16>(p, dev, false, st);
   return pl::launch_few<F16>(p, dev, st);
 }
 
