@@ -132,11 +132,14 @@ DRB_DEV void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
   }
 }
 
+// Sums of bf16 numbers. An infinity less its first term is a NaN; the minimum of that and the largest rest that a finite number leaves is the latter, and infinity
+// and any finite rest add up to the infinity (set to zero by comparisons: 300 fp16 rows 19.2 -> 20.2 us).
+
 // Two f16 numbers as the sum of two pairs of bf16 numbers, exactly (eleven bits; eight and the rest).
 DRB_DEV void split_f16(uint32_t h, uint32_t& hi, uint32_t& lo) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
   const __nv_bfloat162 a = __floats2bfloat162_rn(f.x, f.y);
-  const __nv_bfloat162 b = __floats2bfloat162_rn(f.x - __low2float(a), f.y - __high2float(a));
+  const __nv_bfloat162 b = __hmin2(__floats2bfloat162_rn(f.x - __low2float(a), f.y - __high2float(a)), __float2bfloat162_rn(128.f));
   hi = *reinterpret_cast<const uint32_t*>(&a), lo = *reinterpret_cast<const uint32_t*>(&b);
 }
 
@@ -148,6 +151,7 @@ DRB_DEV void split3(const float4& v, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(r.x, r.y), c = __floats2bfloat162_rn(r.z, r.w);
     b0[l] = *reinterpret_cast<const uint32_t*>(&a), b1[l] = *reinterpret_cast<const uint32_t*>(&c);
     r = make_float4(r.x - __low2float(a), r.y - __high2float(a), r.z - __low2float(c), r.w - __high2float(c));
+    if (l == 0) r = make_float4(fminf(r.x, 0x1p119f), fminf(r.y, 0x1p119f), fminf(r.z, 0x1p119f), fminf(r.w, 0x1p119f));
   }
 }
 
