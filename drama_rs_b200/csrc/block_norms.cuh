@@ -7,7 +7,8 @@
 // Every value is read once and stays in registers through both norms; sums of squares in fp32, by thread, then a butterfly, then the
 // warps in order, so a row's result does not depend on how many rows there are. Bound by HBM for many rows (4 + 4 bytes of x a value
 // beside o and h), by the launch and two block-wide sums for few. Queued: 8192 rows of 2048 33.9 us (5.9 TB/s, 0.91 of a copy's rate; rows through registers,
-// one ahead, 40.8), 300 rows 3.6, one row 2.3; 777 rows of 1501, whose values are loaded one by one, 8.4.
+// one ahead, 40.8), 300 rows 3.6, one row 2.4; 777 rows of 1501, whose values are loaded one by one, 8.5: two such rows in 96 registers spill 124 to 152 bytes. Beyond 2048 columns a
+// multiprocessor has one block: 1500 rows of 8192 29.0, 3000 of 4096 32.0, 6000 of 2052 46.2 (22.5 us of bytes each), 6000 of 2049, one by one, 134.
 #pragma once
 
 #include <type_traits>

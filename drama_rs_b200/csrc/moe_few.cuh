@@ -22,7 +22,7 @@
 // the largest of the 64, as fp32 has it), one column a digit. Sums over 64 inputs are exact integers; scale, min and the digits'
 // weights are applied in fp32. Int4 costs three logic operations per eight weights this way.
 //
-// Queued, 256 experts, top 8: 1 token 18.7 us (18 MB), 5 tokens 30.2 (71 MB), 16 tokens 53.0 (185 MB; 5.4 TB/s while gate/up runs). Of the 53: logits 4.1,
+// Queued, 256 experts, top 8: 1 token 18.8 us (18 MB; k_moe_stack takes 10.9 for it), 5 tokens 30.0 (71 MB), 16 tokens 52.8 (185 MB; 5.4 TB/s while gate/up runs). Of the 53: logits 4.1,
 // routing and runs 4, first weights and digits 3, gate/up 19, hand-over of the activations 4, down 9, last block 3, combine and launch 6. With a dozen
 // runtime divisions on a thread's way 16 tokens took 1 us more, with a fence a tile instead of one a block and equal counts of tiles a block 94 in all.
 //

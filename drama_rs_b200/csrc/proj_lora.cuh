@@ -16,7 +16,8 @@
 // runs: k_shrink lets this kernel in behind its own wait, so what came before k_shrink is complete.
 //
 // Queued (without adapters in brackets): 1 row of 2048 x 4096 7.2 us (5.4), 17 rows of 8192 x 2048 14.6 (8.8), 64 rows of 4096 x 2048 and as many adapters 17.6
-// (9.5). A step of 17 rows takes 0.8 us, of which mma.sync, conversion and reads of shared memory would each take half alone. A pass takes up to 32 rows.
+// (10.9). A step of 17 rows takes 0.8 us, of which mma.sync, conversion and reads of shared memory would each take half alone; no unit is busy for more than 0.4 of
+// the time, so what bounds it is a warp's way through its step, one after another with three slots. A pass takes up to 32 rows.
 #pragma once
 
 #include "common.cuh"

@@ -5,10 +5,10 @@
 // A code becomes a 16-bit number exactly, so the operand carries no scale: the multiplications of each 128 inputs have an
 // accumulator of their own (two, in turns), and the epilogue warps sum scale * accumulator in fp32 as they complete. An adapter of the
 // tile's rows is one more stretch of inputs: its rows of B as the A operand, v (zero in other adapters' rows) as B operand in
-// three bf16 terms, 24 bits; the accumulator joins with a factor of one. Bound by the conversion's issue slots, two instructions a
-// weight (bf16; fp16 one and a quarter) beside its loads and stores: 128 x 128 codes take a multiprocessor about 350 cycles, the
-// multiplications of nc = 80 take 160. Queued, 4096 x 2048, 300 rows: 12.4 us, with 3 adapters of rank 64 19.3; 8192 x 2048, 2048 rows: 133 us (0.52 PFLOP/s),
-// with three adapters of rank 16 159 (one tile a block: 168).
+// three bf16 terms, 24 bits; the accumulator joins with a factor of one. 128 inputs of a tile take 0.49 us with nc = 16 and 0.55 with 80, some 1000 cycles. The conversion's
+// instructions, two a weight (bf16; fp16 one and a quarter) beside its loads and stores, fill about 350 of them, the multiplications of nc = 80 160; no unit is
+// near its limit (issue 0.44, integer pipe 0.37), and what the rest is has not been found. Queued, 4096 x 2048, 300 rows: 12.6 us, with 3 adapters of rank 64 19.2;
+// 8192 x 2048, 2048 rows: 133 us (0.52 PFLOP/s), with three adapters of rank 16 160 (one tile a block: 168).
 //
 // Roles, one block of 16 warps per multiprocessor, meeting on mbarriers, every wait bounded: 8 convert warps (two sets that take turns; a
 // thread the 128 codes of one weight row), 4 epilogue warps (a thread one weight row), one warp that issues the multiplications, one that issues the copies (tiled
@@ -372,7 +372,7 @@ static int launch(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
 // Which form: both sides' times in ns, from measurements of 1 to 300 rows, 2048 to 65536 outputs and 2048 to 8192 inputs (within a tenth or two).
 // The mma.sync form takes so many ns a million weights and pass, by its column tiles, and a launch's start for every 32 passes, whose
 // clusters are about what is resident at once; a row's adapter costs it the row's outputs. The tcgen05 form takes
-// 450 ns for 128 inputs of a tile and 1250 for each different adapter of the tile's rows, every wave of tiles. The host does not know how many
+// 450 ns for 128 inputs of a tile (0.49 to 0.55 us where a block has several) and 1250 for each different adapter of the tile's rows, every wave of tiles. The host does not know how many
 // meet in a tile: all that there are, up to 64 rows, which are likely to be as many requests; a quarter of them beyond, where neighbours are
 // likely to be of one. Measured, mma.sync / tcgen05, us: 8192 x 2048 24 rows 9.0 / 10.1, 48 rows 16.2 / 11.1; 32768 x 2048 24 rows 27 / 19; 2048 x 4096 64
 // rows 10.9 / 18.7; 8192 x 2048, 48 rows of 8 adapters 25.3 / 22.7, of 16 25.4 / 34.9.

@@ -362,7 +362,8 @@ class MoeStackDecoder:
 class MoeBatchDecoder:
     """Several requests decoding together over a stack of MoE layers: x[r] <- x[r] + moe_l(rmsnorm(x[r])) for each layer, one
     kernel a layer (drb_moe_few). The batch has room for `streams` requests; rows that `set_live` switches off cost no expert and stay as they are,
-    also in a captured step. Results of a row do not depend on the others beyond the order of fp32 sums."""
+    also in a captured step. Results of a row do not depend on the others beyond the order of fp32 sums. int4 experts only; for one request
+    alone `MoeDecoder` and `MoeStackDecoder` are faster."""
 
     def __init__(self, layers: list[MoeLayer], streams: int, topk: int = 8, eps: float = 1e-6, st: Stream | None = None) -> None:
         self.l = ffi.lib()
