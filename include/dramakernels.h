@@ -315,8 +315,8 @@ int drb_moe_few(const drb_moe_layer* w, const float* x, float* y, const uint8_t*
  * adapter_of and v may be NULL) is the projection alone; adapters of a smaller rank are padded with zeros. Weights are not rounded: codes meet x
  * exactly, sums over the 128 inputs of a scale and everything behind them are f32. Two launches (one without adapters).
  * No row depends on another one, nor on another adapter than its own (a NaN there stays with its rows).
- * An infinite input, or an A x that overflows, reaches the row's outputs as the formula has it; an infinity in an adapter's a or b, or an A x between
- * bf16's largest number and fp32's, makes infinities or NaNs of the outputs that it enters.
+ * An infinite input, or an A x that overflows, reaches the row's outputs as the formula has it, adapters of b below 512 in size taken; an infinity in a or b,
+ * or an A x between bf16's largest number and fp32's, makes infinities or NaNs of the outputs that it enters. NaNs stay NaNs.
  * k a multiple of 128 up to 8192, rank a multiple of 8 up to 64, n >= 1, rows <= 65535 * 64, else -1 (also on a device that runs no cluster of blocks); w, x, a, b and v 16-byte aligned, else -3
  * (also when the driver refuses a tensor map). w and s are read ahead of the launch before and must not be its work; everything else may be. */
 int drb_proj_q8_lora(const int8_t* w, const dr_half* s, const void* x, int x_type, const dr_bf16* a, const dr_bf16* b, const float* scale,

@@ -50,3 +50,17 @@ def test_a_first_half_that_overflows(rows, n, x_type):
     assert (z[1] == float("inf")).all()
     others = [r for r in range(rows) if r != 1]
     assert torch.equal(z[others], y[others])
+
+
+@pytest.mark.parametrize("bad", [float("-inf"), float("nan")])
+@pytest.mark.parametrize("x_type", [1, 2])
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_a_negative_infinity_and_a_nan(rows, n, x_type, bad):
+    t = case(rows, n, x_type)
+    t["b"][:, :, 0] = 500  # beside the largest rest that a second term may be: finite
+    y = run(t)
+    t["x"][1, AT] = bad
+    z = run(t)
+    assert torch.isnan(z[1]).all() if bad != bad else (z[1] == bad).all()
+    others = [r for r in range(rows) if r != 1]
+    assert torch.equal(z[others], y[others])
