@@ -58,7 +58,7 @@ DRB_DEV void linger() {
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Maps maps, pl::Args p, int nc, int tiles) {
+__global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Maps maps, pl::Args p, int nc, int each, int tiles) {
   extern __shared__ unsigned char dyn_raw[];
   unsigned char* dyn = dyn_raw + (-smem_u32(dyn_raw) & 1023u);
   Ctl& ctl = *reinterpret_cast<Ctl*>(dyn);
@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(640, 1) k_proj_rows(const __grid_constant__ Ma
   unsigned char* xst = raw + NRAW * RAW_BYTES;
   const int box = nc * 128, xstage = 3 * box;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = p.k >> 7, row0 = (int)blockIdx.y * nc, cols = min(nc, p.rows - row0);
+  const int groups = p.k >> 7, row0 = (int)blockIdx.y * each, cols = min(each, p.rows - row0);
   unsigned spent = 0;  // a wait of this thread ran out: none spins again
   const int first = (int)blockIdx.x, step = (int)gridDim.x, mine = first < tiles ? (tiles - first + step - 1) / step : 0;
 
@@ -364,8 +364,9 @@ static int launch(const pl::Args& p, const DrbDevice& dev, cudaStream_t st) {
   if (!e) e = map_2d(&maps.x, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.x, p.k, p.rows, (uint64_t)p.k * 2, 64, nc);
   if (e) return e;
   if (p.rank > 0) pl::launch_shrink<F16>(p, dev, true, st);
-  const int each = dev.sms / passes;
-  drb_launch(k_proj_rows<F16>, dim3(each < 1 ? 1 : each < tiles ? each : tiles, passes), dim3(THREADS), smem_bytes(nc), st, dev.pdl, maps, p, nc, tiles);
+  // A pass has its blocks for good, so the rows are shared out evenly, not nc a pass: 100 rows of 64 adapters were 64 and 36, with as many adapters
+  const int blocks = dev.sms / passes, each = (p.rows + passes - 1) / passes;
+  drb_launch(k_proj_rows<F16>, dim3(blocks < 1 ? 1 : blocks < tiles ? blocks : tiles, passes), dim3(THREADS), smem_bytes(nc), st, dev.pdl, maps, p, nc, each, tiles);
   return 0;
 }
 

@@ -118,7 +118,8 @@ def test_several_tiles_without_adapters(rows, n, k, x_type):
 # to the other at a tile's end), ranks from the smallest to the largest, rows of one adapter behind one another and mixed
 BESIDE = [(16, 75_700, 768, 1, 8), (16, 75_700, 8192, 1, 16), (16, 75_700, 8192, 2, 64), (16, 75_700, 8192, 3, 24), (80, 60_001, 768, 1, 64),
           (80, 60_001, 768, 2, 16), (80, 60_001, 768, 3, 40), (80, 57_000, 8192, 1, 16), (80, 57_000, 8192, 2, 8), (80, 57_000, 8192, 3, 64),
-          (150, 57_003, 2048, 3, 16), (300, 40_000, 1024, 9, 32)]
+          (150, 57_003, 2048, 3, 16), (300, 40_000, 1024, 9, 32),
+          (100, 32_768, 2048, 64, 16), (81, 40_001, 640, 12, 8), (161, 40_001, 1024, 5, 24)]  # and rows that a pass's columns do not divide
 
 
 @pytest.mark.parametrize("x_type", [1, 2])
