@@ -7,8 +7,8 @@
 // tile's rows is one more stretch of inputs: its rows of B as the A operand, v (zero in other adapters' rows) as B operand in
 // three bf16 terms, 24 bits; the accumulator joins with a factor of one. 128 inputs of a tile take 0.49 us with nc = 16 and 0.55 with 80, some 1000 cycles. The conversion's
 // instructions, two a weight (bf16; fp16 one and a quarter) beside its loads and stores, fill about 350 of them, the multiplications of nc = 80 160; no unit is
-// near its limit (issue 0.44, integer pipe 0.37), and what the rest is has not been found. Queued, 4096 x 2048, 300 rows: 12.6 us, with 3 adapters of rank 64 19.2;
-// 8192 x 2048, 2048 rows: 133 us (0.52 PFLOP/s), with three adapters of rank 16 160 (one tile a block: 168).
+// near its limit (issue 0.44, integer pipe 0.37), and what the rest is has not been found. Queued, 4096 x 2048, 300 rows: 12.6 us, with 3 adapters of rank 64 17.8;
+// 8192 x 2048, 2048 rows: 133 us (0.52 PFLOP/s), with three adapters of rank 16 162 (one tile a block: 168).
 //
 // Roles, one block of 16 warps per multiprocessor, meeting on mbarriers, every wait bounded: 8 convert warps (two sets that take turns; a
 // thread the 128 codes of one weight row), 4 epilogue warps (a thread one weight row), one warp that issues the multiplications, one that issues the copies (tiled
